@@ -43,11 +43,13 @@ typedef struct Rib200Status {
 
 /* cpp/include/raftinfer/tensor.h:10-15 */
 enum { RIB200_DTYPE_F32 = 1, RIB200_DTYPE_F16 = 2, RIB200_DTYPE_BF16 = 3 };
+enum { RIB200_DTYPE_E4M3 = 4 }; /* no counterpart in the reference; an output of rib200_residual_rms_norm */
 /* cpp/execution/qwen35_execution_policy.hpp:7-27 */
 enum { RIB200_ATTENTION_MATERIALIZED_REFERENCE = 0, RIB200_ATTENTION_ONLINE_TILED = 1 };
 enum { RIB200_DECODE_AUTO_SELECT = 0, RIB200_DECODE_SINGLE_BLOCK = 1, RIB200_DECODE_SPLIT_K_256 = 2,
        RIB200_DECODE_SPLIT_K_512 = 3 };
 enum { RIB200_KV_CACHE_F32 = 0, RIB200_KV_CACHE_BF16 = 1 };
+enum { RIB200_KV_CACHE_E4M3 = 2 }; /* no counterpart in the reference; taken by the rib200_kv_* calls alone */
 enum { RIB200_KV_LAYOUT_TOKEN_MAJOR = 0, RIB200_KV_LAYOUT_HEAD_MAJOR = 1 };
 /* cpp/kernels/qwen35_delta.cuh:31-35 */
 enum { RIB200_DELTA_SCHEDULE_CURRENT = 0, RIB200_DELTA_SCHEDULE_PREFILL_SM120 = 1,
@@ -398,6 +400,85 @@ Rib200Status rib200_online_attention_decode_early_kv_fetch(const void *query, co
                                                            int32_t activation_dtype, uint8_t cache_dtype,
                                                            uint8_t cache_layout, const Rib200OnlineDecodePlan *plan,
                                                            void *stream);
+
+/* ---- attention over a BF16 or 8-bit KV cache, whole or windowed (no counterpart in the reference) ------------
+ * The calls below take two kinds of cache, both [K, V][kv head][...] with head_dim 256:
+ *   RIB200_KV_CACHE_BF16  rows as everywhere else in this library, [2][kv_heads][max_context_tokens][256];
+ *   RIB200_KV_CACHE_E4M3  [2][kv_heads][ceil(max_context_tokens / 16)] blocks of RIB200_KV8_BLOCK_BYTES: 16 rows of 256
+ *                         e4m3 codes, the block's FP32 scale, 12 bytes that are not used.  A row's value is code * scale.
+ * A page of the paged calls is a cache of 256 tokens of the same kind.
+ *
+ * Scales are powers of two: 2^e with e in [-100, 119], the least for which the largest finite magnitude of the block is
+ * at most 448 * 2^e, so that dividing by one is exact and a code is its value rounded once, to nearest even.  Infinities
+ * become +-448 scales, a not-a-number stays one.  Rows that are written into a block behind rows that are there already
+ * keep the block's scale, or raise it when they need a larger one; the rows in front are then rounded to the new scale, which
+ * changes only what falls under its smallest normal code (2^-6).  Rows have to be written in order, from row 0 on.
+ *
+ * Attention reads what the cache holds: the new tokens' rows are stored first, and 8-bit rows are used as rounded.  A query
+ * at position p sees the tokens j <= p with j > p - window_tokens or j < sink_tokens; window_tokens == 0 is the whole
+ * context.  What is not visible may hold anything in a single-token call; in a prompt call the rows that its first token
+ * does not see (neither a sink nor in its window) may hold anything in an 8-bit or paged cache and have to be finite in a
+ * contiguous BF16 one.  Pages with no visible row are not looked up.  Outputs are out = (attention) * sigmoid(gate).
+ * Activations (query, key, value, gate, output) are BF16 or FP32; a prompt call rounds FP32 queries to BF16, and FP32
+ * keys and values to the cache's type; a single-token call rounds keys and values alone. */
+enum { RIB200_KV8_BLOCK_TOKENS = 16, RIB200_KV8_BLOCK_BYTES = 4112 };
+/* A batch entry of rib200_kv_batched_decode and rib200_kv_paged_decode with this position is skipped: nothing is stored and
+ * its output row stays as it is. */
+#define RIB200_NO_POSITION 0xFFFFFFFFu
+
+/* Bytes of one sequence's cache; a page is rib200_kv_cache_bytes(kv_heads, 256, ...).  BF16 or E4M3. */
+Rib200Status rib200_kv_cache_bytes(size_t kv_heads, size_t max_context_tokens, uint8_t cache_dtype, size_t *bytes);
+/* Workspace of the prompt calls: the rows that the chunk sees, in BF16.  0 for a contiguous BF16 cache (paged == 0). */
+Rib200Status rib200_kv_prefill_workspace_bytes(const Rib200AttentionShape *shape, size_t window_tokens,
+                                               size_t sink_tokens, uint8_t cache_dtype, int32_t paged, size_t *bytes);
+/* Workspace of the single-token calls, the same for every batch and length. */
+Rib200Status rib200_kv_decode_workspace_bytes(size_t *bytes);
+
+/* A chunk of shape->tokens >= 1 tokens behind shape->past_tokens on one sequence's cache: query, gate, output
+ * [tokens][query_heads][256], key, value [tokens][kv_heads][256], query_heads a multiple of kv_heads. */
+Rib200Status rib200_kv_attention_prefill(const void *query, const void *key, const void *value, const void *gate,
+                                         void *output, void *kv_cache, size_t kv_cache_bytes, void *workspace,
+                                         size_t workspace_bytes, const Rib200AttentionShape *shape,
+                                         size_t window_tokens, size_t sink_tokens, int32_t activation_dtype,
+                                         uint8_t cache_dtype, void *stream);
+/* The same on a sequence whose rows lie in pages of 256 tokens: block_table[b] (device memory, max_blocks entries) names
+ * the page of rows [256 b, 256 b + 256); shape->max_context_tokens is 256 * max_blocks.  A page index outside the pool
+ * sets RIB200_DEVICE_PAGE_OUT_OF_RANGE; such a page is neither read nor written and the output is undefined. */
+Rib200Status rib200_kv_paged_prefill(const void *query, const void *key, const void *value, const void *gate, void *output,
+                                     void *page_pool, size_t pool_pages, const uint32_t *block_table, size_t max_blocks,
+                                     void *workspace, size_t workspace_bytes, const Rib200AttentionShape *shape,
+                                     size_t window_tokens, size_t sink_tokens, int32_t activation_dtype,
+                                     uint8_t cache_dtype, void *stream);
+/* One token for each sequence of a batch, as rib200_batched_decode_attention: query, gate, output
+ * [batch][query_heads][256], key, value [batch][kv_heads][256]; 1 to 4 query heads per KV head.  kv_caches,
+ * max_context_tokens and positions are device arrays of `batch` entries; a position outside its cache (other than
+ * RIB200_NO_POSITION) sets RIB200_DEVICE_POSITION_OUT_OF_RANGE and the entry is skipped.  Two entries may share rows that
+ * both only read, not the row (8-bit: the block) that either writes. */
+Rib200Status rib200_kv_batched_decode(const void *query, const void *key, const void *value, const void *gate,
+                                      void *output, void *const *kv_caches, const uint32_t *max_context_tokens,
+                                      const uint32_t *positions, size_t batch, size_t query_heads, size_t kv_heads,
+                                      size_t window_tokens, size_t sink_tokens, int32_t activation_dtype,
+                                      uint8_t cache_dtype, void *workspace, size_t workspace_bytes, void *stream);
+/* Its paged form, as rib200_paged_decode_attention. */
+Rib200Status rib200_kv_paged_decode(const void *query, const void *key, const void *value, const void *gate, void *output,
+                                    void *page_pool, size_t pool_pages, const uint32_t *block_tables,
+                                    size_t max_blocks_per_sequence, const uint32_t *positions, size_t batch,
+                                    size_t query_heads, size_t kv_heads, size_t window_tokens, size_t sink_tokens,
+                                    int32_t activation_dtype, uint8_t cache_dtype, void *workspace,
+                                    size_t workspace_bytes, void *stream);
+
+/* ---- the row step in front of a layer's projections -----------------------------------------------------------
+ * qwen35_rms_norm behind the executor's residual addition (cpp/kernels/qwen35_primitives.cu:118-160) as one call, with an
+ * output in 8 bits where the projection takes one: h = input + residual in FP32 (residual may be NULL),
+ * residual_out = h in `dtype` (may be NULL; may be `residual` or `input` itself), y = h / sqrt(mean(h^2) + epsilon) * weight.
+ * output_dtype == dtype: output = y, scales NULL, group_columns 0.  RIB200_DTYPE_E4M3: output holds codes [rows][columns]
+ * and scales (FP32) [rows][columns / group_columns], the powers of two of the 8-bit cache for each group of 32 or 128
+ * columns of a row; group_columns == 0 is one scale for the row.  dtype FP32, BF16 or FP16; weight FP32 or BF16;
+ * columns a multiple of 8 (of group_columns) up to 16384. */
+Rib200Status rib200_residual_rms_norm(const void *input, const void *residual, const void *weight, void *output,
+                                      float *scales, void *residual_out, size_t rows, size_t columns,
+                                      size_t group_columns, float epsilon, int32_t dtype, int32_t weight_dtype,
+                                      int32_t output_dtype, void *stream);
 
 /* Reads and clears the status word the kernels of this library set on the current device.  It
  * synchronises `stream` first, so it is not for use inside a graph capture. */

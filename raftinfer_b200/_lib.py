@@ -112,6 +112,17 @@ PROTOTYPES = {
                                                       C.c_int32, C.c_uint8, C.c_uint8,
                                                       C.POINTER(OnlineDecodePlan), vp],
     "rib200_paged_decode_attention": [vp, vp, vp, vp, vp, vp, sz, vp, sz, vp, sz, vp, sz, vp],
+    "rib200_kv_cache_bytes": [sz, sz, C.c_uint8, C.POINTER(sz)],
+    "rib200_kv_prefill_workspace_bytes": [C.POINTER(AttentionShape), sz, sz, C.c_uint8, C.c_int32, C.POINTER(sz)],
+    "rib200_kv_decode_workspace_bytes": [C.POINTER(sz)],
+    "rib200_kv_attention_prefill": [vp, vp, vp, vp, vp, vp, sz, vp, sz, C.POINTER(AttentionShape), sz, sz, C.c_int32,
+                                    C.c_uint8, vp],
+    "rib200_kv_paged_prefill": [vp, vp, vp, vp, vp, vp, sz, vp, sz, vp, sz, C.POINTER(AttentionShape), sz, sz, C.c_int32,
+                                C.c_uint8, vp],
+    "rib200_kv_batched_decode": [vp, vp, vp, vp, vp, vp, vp, vp, sz, sz, sz, sz, sz, C.c_int32, C.c_uint8, vp, sz, vp],
+    "rib200_kv_paged_decode": [vp, vp, vp, vp, vp, vp, sz, vp, sz, vp, sz, sz, sz, sz, sz, C.c_int32, C.c_uint8, vp, sz,
+                               vp],
+    "rib200_residual_rms_norm": [vp, vp, vp, vp, vp, vp, sz, sz, sz, C.c_float, C.c_int32, C.c_int32, C.c_int32, vp],
     "rib200_device_status": [vp, C.POINTER(C.c_uint32)],
 }
 

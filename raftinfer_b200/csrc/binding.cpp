@@ -249,13 +249,27 @@ using GatedDelta = Entry<rib200_gated_delta, kDelta, P, P, P, P, P, P, P, P, P, 
 using DeltaCore = Entry<rib200_gdn_core, kDelta, P, P, P, P, P, P, P, P, Size, Size, Size, Size, Size, Size, Code, Stream>;
 using BatchedDelta = Entry<rib200_batched_gdn_decode, kDelta, P, P, P, P, P, P, P, Size, Size, Size, Stream>;
 
+using KvPrefill = Entry<rib200_kv_attention_prefill, kAttention, P, P, P, P, P, P, Size, P, Size, AttentionShape, Size, Size,
+                        Code, Byte, Stream>;
+using KvPagedPrefill = Entry<rib200_kv_paged_prefill, kAttention, P, P, P, P, P, P, Size, P, Size, P, Size, AttentionShape,
+                             Size, Size, Code, Byte, Stream>;
+using KvBatchedDecode = Entry<rib200_kv_batched_decode, kAttention, P, P, P, P, P, P, P, P, Size, Size, Size, Size, Size, Code,
+                              Byte, P, Size, Stream>;
+using KvPagedDecode = Entry<rib200_kv_paged_decode, kAttention, P, P, P, P, P, P, Size, P, Size, P, Size, Size, Size, Size,
+                            Size, Code, Byte, P, Size, Stream>;
+using ResidualNorm = Entry<rib200_residual_rms_norm, kAttention, P, P, P, P, P, P, Size, Size, Size, Float, Code, Code, Code,
+                           Stream>;
+
 using FastCall = PyObject *(*)(PyObject *, PyObject *const *, Py_ssize_t);
 struct Row {
-  const char *name;
+  const char *name; // of the entry point
+  const char *as;   // of the Python function
   FastCall call;
   void (*bind)(void *, PyObject *);
 };
-template <class E> constexpr Row row(const char *name) { return Row{name, &E::call, &E::bind}; }
+template <class E> constexpr Row row(const char *name, const char *as = nullptr) {
+  return Row{name, as != nullptr ? as : name, &E::call, &E::bind};
+}
 const Row kRows[] = {
     row<CausalAttention>("rib200_causal_attention"),
     row<Prefill>("rib200_online_attention_prefill"),
@@ -270,7 +284,47 @@ const Row kRows[] = {
     row<DeltaCore>("rib200_gdn_core"),
     row<BatchedDelta>("rib200_batched_gdn_decode"),
 };
+// Entry points without a counterpart in the reference that came later; they go by the names they have in kernels.py.
+const Row kMoreRows[] = {
+    row<KvPrefill>("rib200_kv_attention_prefill", "kv_attention_prefill"),
+    row<KvPagedPrefill>("rib200_kv_paged_prefill", "kv_paged_prefill"),
+    row<KvBatchedDecode>("rib200_kv_batched_decode", "kv_batched_decode"),
+    row<KvPagedDecode>("rib200_kv_paged_decode", "kv_paged_decode"),
+    row<ResidualNorm>("rib200_residual_rms_norm", "residual_rms_norm"),
+};
 constexpr std::size_t kRowCount = sizeof(kRows) / sizeof(kRows[0]);
+constexpr std::size_t kMoreCount = sizeof(kMoreRows) / sizeof(kMoreRows[0]);
+
+bool bind_row(const Row &row, PyObject *address_of) {
+  PyObject *name = PyUnicode_FromString(row.name);
+  PyObject *address = name != nullptr ? PyObject_CallOneArg(address_of, name) : nullptr;
+  if (address == nullptr) {
+    Py_XDECREF(name);
+    return false;
+  }
+  void *value = PyLong_AsVoidPtr(address);
+  Py_DECREF(address);
+  if (value == nullptr) {
+    if (!PyErr_Occurred()) {
+      PyErr_Format(PyExc_ImportError, "%s has no address", row.name);
+    }
+    Py_DECREF(name);
+    return false;
+  }
+  row.bind(value, name);
+  Py_DECREF(name);
+  return true;
+}
+
+// bind_more(address of a name): the entry points of kMoreRows
+PyObject *bind_more(PyObject *, PyObject *address_of) {
+  for (const Row &row : kMoreRows) {
+    if (!bind_row(row, address_of)) {
+      return nullptr;
+    }
+  }
+  Py_RETURN_NONE;
+}
 
 // bind(address of a name, through_ctypes, attention error, gated-delta error)
 PyObject *bind(PyObject *, PyObject *const *args, Py_ssize_t count) {
@@ -279,23 +333,9 @@ PyObject *bind(PyObject *, PyObject *const *args, Py_ssize_t count) {
     return nullptr;
   }
   for (const Row &row : kRows) {
-    PyObject *name = PyUnicode_FromString(row.name);
-    PyObject *address = name != nullptr ? PyObject_CallOneArg(args[0], name) : nullptr;
-    if (address == nullptr) {
-      Py_XDECREF(name);
+    if (!bind_row(row, args[0])) {
       return nullptr;
     }
-    void *value = PyLong_AsVoidPtr(address);
-    Py_DECREF(address);
-    if (value == nullptr) {
-      if (!PyErr_Occurred()) {
-        PyErr_Format(PyExc_ImportError, "%s has no address", row.name);
-      }
-      Py_DECREF(name);
-      return nullptr;
-    }
-    row.bind(value, name);
-    Py_DECREF(name);
   }
   Py_XSETREF(g_through_ctypes, Py_NewRef(args[1]));
   Py_XSETREF(g_errors[kAttention], Py_NewRef(args[2]));
@@ -303,16 +343,23 @@ PyObject *bind(PyObject *, PyObject *const *args, Py_ssize_t count) {
   Py_RETURN_NONE;
 }
 
-PyMethodDef g_methods[kRowCount + 2];
+PyMethodDef g_methods[kRowCount + kMoreCount + 3];
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_call", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 
 } // namespace
 
 PyMODINIT_FUNC PyInit__call() {
   g_methods[0] = {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(bind)), METH_FASTCALL, nullptr};
-  for (std::size_t i = 0; i < kRowCount; ++i) {
-    g_methods[i + 1] = {kRows[i].name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(kRows[i].call)),
-                        METH_FASTCALL, nullptr};
+  g_methods[1] = {"bind_more", bind_more, METH_O, nullptr};
+  std::size_t at = 2;
+  auto add = [&](const Row &row) {
+    g_methods[at++] = {row.as, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(row.call)), METH_FASTCALL, nullptr};
+  };
+  for (const Row &row : kRows) {
+    add(row);
+  }
+  for (const Row &row : kMoreRows) {
+    add(row);
   }
   g_data_ptr = PyUnicode_InternFromString("data_ptr");
   g_cuda_stream = PyUnicode_InternFromString("cuda_stream");

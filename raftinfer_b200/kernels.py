@@ -24,10 +24,14 @@ except ImportError as error:
 
 # RaftInferDataType, cpp/include/raftinfer/tensor.h:10-15
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 1, 2, 3
+DTYPE_E4M3 = 4  # an output of residual_rms_norm
 # cpp/execution/qwen35_execution_policy.hpp:7-27
 MATERIALIZED_REFERENCE, ONLINE_TILED = 0, 1
 AUTO_SELECT, SINGLE_BLOCK, SPLIT_K_256, SPLIT_K_512 = 0, 1, 2, 3
 KV_F32, KV_BF16 = 0, 1
+KV_E4M3 = 2  # taken by the kv_* calls
+KV8_BLOCK_TOKENS, KV8_BLOCK_BYTES = 16, 4112
+NO_POSITION = 0xFFFFFFFF
 TOKEN_MAJOR, HEAD_MAJOR = 0, 1
 # status codes, cpp/include/raftinfer/status.h:7-20
 OK, INVALID_ARGUMENT, UNAVAILABLE, CUDA_ERROR, INTERNAL, UNSUPPORTED, RESOURCE_EXHAUSTED = range(7)
@@ -98,6 +102,7 @@ def _through_ctypes(name, *arguments):
 # The launchers go through native functions (csrc/binding.cpp); sizes, plans and the rest through ctypes.
 _call.bind(lambda name: C.cast(getattr(lib, name), C.c_void_p).value, _through_ctypes, Qwen35PrimitiveError,
            Qwen35DeltaError)
+_call.bind_more(lambda name: C.cast(getattr(lib, name), C.c_void_p).value)
 
 
 @dataclass(frozen=True)
@@ -382,6 +387,68 @@ def paged_decode_attention(query, key, value, gate, output, page_pool, pool_page
     tables (uint32, device memory)."""
     _call.rib200_paged_decode_attention(query, key, value, gate, output, page_pool, pool_pages, block_tables,
                                         max_blocks_per_sequence, positions, batch, workspace, workspace_bytes, stream)
+
+
+# ---- attention over a BF16 or 8-bit cache, whole or windowed; no counterpart in the reference --------------------
+def kv_cache_bytes(kv_heads, max_context_tokens, cache_dtype):
+    out = C.c_size_t()
+    _check(lib.rib200_kv_cache_bytes(kv_heads, max_context_tokens, cache_dtype, C.byref(out)))
+    return out.value
+
+
+def kv_prefill_workspace_bytes(shape, window_tokens, sink_tokens, cache_dtype, paged=False):
+    out = C.c_size_t()
+    s = shape.c()
+    _check(lib.rib200_kv_prefill_workspace_bytes(C.byref(s), window_tokens, sink_tokens, cache_dtype, 1 if paged else 0,
+                                                 C.byref(out)))
+    return out.value
+
+
+def kv_decode_workspace_bytes():
+    out = C.c_size_t()
+    _check(lib.rib200_kv_decode_workspace_bytes(C.byref(out)))
+    return out.value
+
+
+def kv_attention_prefill(query, key, value, gate, output, kv_cache, kv_cache_bytes, workspace, workspace_bytes, shape,
+                         window_tokens, sink_tokens, activation_dtype, cache_dtype, stream):
+    """A chunk of a prompt on one sequence's BF16 or 8-bit cache; visible are the last `window_tokens` tokens (0: all)
+    and the first `sink_tokens`.  See include/rib200.h for the caches and what is rounded."""
+    _call.kv_attention_prefill(query, key, value, gate, output, kv_cache, kv_cache_bytes, workspace, workspace_bytes, shape,
+                               window_tokens, sink_tokens, activation_dtype, cache_dtype, stream)
+
+
+def kv_paged_prefill(query, key, value, gate, output, page_pool, pool_pages, block_table, max_blocks, workspace,
+                     workspace_bytes, shape, window_tokens, sink_tokens, activation_dtype, cache_dtype, stream):
+    """The chunk on a sequence whose rows lie in pages of 256 tokens."""
+    _call.kv_paged_prefill(query, key, value, gate, output, page_pool, pool_pages, block_table, max_blocks, workspace,
+                           workspace_bytes, shape, window_tokens, sink_tokens, activation_dtype, cache_dtype, stream)
+
+
+def kv_batched_decode(query, key, value, gate, output, kv_caches, max_context_tokens, positions, batch, query_heads,
+                      kv_heads, window_tokens, sink_tokens, activation_dtype, cache_dtype, workspace, workspace_bytes,
+                      stream):
+    """One token for each sequence of a batch on BF16 or 8-bit caches; a position of NO_POSITION skips its entry."""
+    _call.kv_batched_decode(query, key, value, gate, output, kv_caches, max_context_tokens, positions, batch, query_heads,
+                            kv_heads, window_tokens, sink_tokens, activation_dtype, cache_dtype, workspace, workspace_bytes,
+                            stream)
+
+
+def kv_paged_decode(query, key, value, gate, output, page_pool, pool_pages, block_tables, max_blocks_per_sequence,
+                    positions, batch, query_heads, kv_heads, window_tokens, sink_tokens, activation_dtype, cache_dtype,
+                    workspace, workspace_bytes, stream):
+    """The batched step over a pool of 256-token pages named by per-sequence block tables (uint32, device memory)."""
+    _call.kv_paged_decode(query, key, value, gate, output, page_pool, pool_pages, block_tables, max_blocks_per_sequence,
+                          positions, batch, query_heads, kv_heads, window_tokens, sink_tokens, activation_dtype, cache_dtype,
+                          workspace, workspace_bytes, stream)
+
+
+def residual_rms_norm(input, residual, weight, output, scales, residual_out, rows, columns, group_columns, epsilon, dtype,
+                      weight_dtype, output_dtype, stream):
+    """Residual addition and RMS norm of hidden rows, with an output in `dtype` or in 8 bits with a scale for each group of
+    columns.  `residual`, `scales` and `residual_out` may be None as include/rib200.h says."""
+    _call.residual_rms_norm(input, residual, weight, output, scales, residual_out, rows, columns, group_columns, epsilon,
+                            dtype, weight_dtype, output_dtype, stream)
 
 
 # ---- gated delta ---------------------------------------------------------------------------------

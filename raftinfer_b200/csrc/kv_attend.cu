@@ -127,77 +127,7 @@ template <bool F32> __global__ void __launch_bounds__(128) kv_attend_kernel(cons
   }
 }
 
-// grid = (sequences, KV heads, 2), a warp: the new row of a sequence into its cache
-template <bool F32> __global__ void __launch_bounds__(32) kv_append_kernel(const KvDecodeArgs a, unsigned int *status) {
-  grid_dependency_wait();
-  grid_dependents_may_launch();
-  const std::uint32_t sequence = blockIdx.x, head = blockIdx.y, is_value = blockIdx.z;
-  const std::uint32_t pos = a.positions[sequence];
-  std::uint32_t why;
-  if (!kv_servable(a.caches, sequence, pos, why)) {
-    if (why != 0 && threadIdx.x == 0) {
-      atomicOr(status, why);
-    }
-    return;
-  }
-  const KvView view = kv_view(a.caches, sequence);
-  unsigned char *plane = view.plane(is_value, head, pos);
-  if (plane == nullptr) {
-    return; // reported by the reader
-  }
-  float x[8];
-  load8<F32>(is_value != 0 ? a.value : a.key,
-             (static_cast<std::size_t>(sequence) * a.caches.kv_heads + head) * kKvHeadDim + threadIdx.x * 8, x);
-  const std::uint32_t row = view.row_in_plane(pos);
-  if (!view.eight_bit) {
-    __nv_bfloat16 *at = reinterpret_cast<__nv_bfloat16 *>(plane) + static_cast<std::size_t>(row) * kKvHeadDim + threadIdx.x * 8;
-    for (int e = 0; e < 8; ++e) {
-      at[e] = __float2bfloat16_rn(x[e]);
-    }
-    return;
-  }
-  unsigned char *record = plane + static_cast<std::size_t>(row / kKv8BlockTokens) * kKv8BlockBytes;
-  float amax = 0.0F;
-  for (int e = 0; e < 8; ++e) {
-    amax = fmaxf(amax, kv8_finite_magnitude(x[e]));
-  }
-  for (int step = 16; step > 0; step /= 2) {
-    amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFU, amax, step));
-  }
-  float *stored = reinterpret_cast<float *>(record + kKv8CodeBytes);
-  const float before = row % kKv8BlockTokens != 0 ? *stored : 0.0F;
-  __syncwarp();
-  const float scale = fmaxf(kv8_scale(amax), before);
-  const float inverse = kv8_inverse(scale);
-  if (threadIdx.x == 0) {
-    *stored = scale;
-  }
-  if (scale != before) {
-    for (std::uint32_t i = threadIdx.x; i < (row % kKv8BlockTokens) * kKvHeadDim; i += 32) {
-      record[i] = static_cast<unsigned char>(kv8_codes2(kv8_values2(record[i]).x * (before * inverse), 0.0F));
-    }
-  }
-  for (int e = 0; e < 8; ++e) {
-    record[(row % kKv8BlockTokens) * kKvHeadDim + threadIdx.x * 8 + e] =
-        static_cast<unsigned char>(kv8_codes2(x[e] * inverse, 0.0F));
-  }
-}
-
 } // namespace
-
-std::size_t kv_decode_workspace_bytes() { return 4 << 20; }
-
-void launch_kv_decode(const KvDecodeArgs &a, cudaStream_t stream) {
-  unsigned int *status = device_status_word();
-  const dim3 grid(a.batch, a.caches.kv_heads, 2);
-  AttendArgs p{a.query, a.gate, a.output, a.caches, a.positions, 0, a.query_heads, a.window, a.sinks, status};
-  auto run = [&](auto append, auto attend) {
-    launch_programmatic(append, grid, dim3(32), 0, stream, "KV append launch", a, status);
-    launch_programmatic(attend, dim3(a.batch, a.query_heads), dim3(128), 0, stream, "KV attention launch", p);
-  };
-  a.activations_f32 ? run(kv_append_kernel<true>, kv_attend_kernel<true>)
-                    : run(kv_append_kernel<false>, kv_attend_kernel<false>);
-}
 
 void launch_kv_prefill(const KvPrefillArgs &a, cudaStream_t stream) {
   launch_kv_store(a, stream);

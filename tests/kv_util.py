@@ -121,8 +121,9 @@ def visible(position, window, sinks):
 
 def attention(cache, query, gate, past, window, sinks):
     """Rows query, gate [n, heads, 256] (FP32) at positions past .. in 64 bits: the output; attention of |v| times the gate,
-    which bounds what relative errors of weights do; and the largest sum |q_d k_d| / 16 of a visible key, which bounds what
-    relative errors of products do to a logit."""
+    which bounds what relative errors of weights do; the largest sum |q_d k_d| / 16 of a visible key, which bounds what
+    relative errors of products do to a logit; and the number of visible tokens times the head's largest |v| times two times the
+    gate, which bounds what errors of weights relative to the largest one do."""
     n, heads, _ = query.shape
     group = heads // cache.kv_heads
     tokens = sorted(set().union(*[visible(past + i, window, sinks) for i in (0, n - 1)], range(past, past + n)))
@@ -141,7 +142,8 @@ def attention(cache, query, gate, past, window, sinks):
     out = (weights @ clean).permute(1, 0, 2) * gates
     size = (weights @ clean.abs()).permute(1, 0, 2) * gates
     spread = (q.abs() @ torch.where(held, keys, torch.zeros_like(keys)).abs().transpose(1, 2) / 16.0).masked_fill(~seen, 0.0)
-    return out, size, spread.amax(-1).permute(1, 0)[..., None]
+    total = 2.0 * seen.sum(-1)[:, None, None] * clean.abs().amax((1, 2))[None, :, None] * gates
+    return out, size, spread.amax(-1).permute(1, 0)[..., None], total
 
 
 def normal(seed, *shape):

@@ -86,7 +86,7 @@ class Prompt:
         if check:
             torch.cuda.synchronize()
             assert K.device_status(torch.cuda.current_stream()) == 0
-            out, size, spread = attention(self.model, q, g, past, self.window, self.sinks)
+            out, size, spread, total = attention(self.model, q, g, past, self.window, self.sinks)
             limit = tolerance(out, size, spread, query.dtype, self.dtype == K.DTYPE_F32)
             off = (self.output[:tokens].double() - out).abs()
             assert (off <= limit).all(), (tokens, past, float((off / limit).max()))
@@ -177,8 +177,8 @@ def test_a_prompt_in_chunks_and_then_tokens(kind, paged):
         p.model.store(position, np.stack([k[0].numpy(), v[0].numpy()])[:, :, None])
         p.past += 1
         torch.cuda.synchronize()
-        out, size, spread = attention(p.model, q, g, position, p.window, p.sinks)
-        assert ((output.double() - out).abs() <= token_tolerance(out, size, spread, torch.bfloat16)).all()
+        out, size, spread, total = attention(p.model, q, g, position, p.window, p.sinks)
+        assert ((output.double() - out).abs() <= token_tolerance(out, size, spread, total, torch.bfloat16)).all()
         p.check_cache()
     assert K.device_status(stream) == 0
 

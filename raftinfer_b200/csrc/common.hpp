@@ -144,6 +144,17 @@ struct BatchedDecodeArgs {
 void launch_batched_decode_attention(const BatchedDecodeArgs &args, cudaStream_t stream);
 
 // ---- prefill attention (prefill_attention.cu) -----------------------------------------------
+// Windowed form of the launch: a query at position q sees keys j <= q with j > q - window or j < sinks.
+struct PrefillWindow {
+  std::uint32_t window; // 0: not windowed
+  std::uint32_t sinks;
+  std::uint32_t low;        // first token of the first query's window
+  std::uint32_t seen_sinks; // sinks in front of the last query's window
+  // null, or BF16 [K, V][kv head][staged_rows][256] with tokens [0, seen_sinks) and [low, past + tokens): attention reads this
+  // copy and the chunk's rows in it, and writes no cache
+  void *staged;
+  std::uint32_t staged_rows;
+};
 struct PrefillArgs {
   const void *query;  // [tokens][query_heads][256] activation dtype
   const void *key;    // [tokens][kv_heads][256]
@@ -165,6 +176,7 @@ struct PrefillArgs {
   std::uint32_t output_self; // index of this rank's own buffer
   std::uint32_t output_heads;
   std::uint32_t output_head_offset;
+  PrefillWindow window;
 };
 void launch_prefill_attention(const PrefillArgs &args, cudaStream_t stream);
 // device-side rendezvous of the ranks of one box (peer.cu)

@@ -8,7 +8,7 @@
 // is converted once here and not once for every query tile and head there.
 // Bytes: inputs and cache rows once, workspace rows once; bound by memory, or by launch latency for short chunks.
 
-#include "kv_store.hpp"
+#include "kv_cache.hpp"
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -17,6 +17,18 @@
 
 namespace rib200 {
 namespace {
+
+struct KvStoreArgs {
+  const void *key, *value;
+  KvCaches caches;
+  std::uint32_t tokens, past;
+  std::uint32_t sink_blocks;  // blocks of 16 tokens [0, sink_blocks), then [window_block, ...)
+  std::uint32_t window_block;
+  std::uint32_t seen_sinks, seen_low;
+  void *staged; // BF16 [K, V][kv head][staged_rows][256]: tokens [0, seen_sinks), then from seen_low on
+  std::uint32_t staged_rows;
+  unsigned int *status;
+};
 
 constexpr int kThreads = 128; // eight threads a row, which take 8 of every 64 dims
 constexpr int kPieces = 4;
@@ -182,8 +194,6 @@ template <bool F32, bool EightBit> __global__ void __launch_bounds__(kThreads) k
   }
 }
 
-} // namespace
-
 void launch_kv_store(const KvPrefillArgs &a, cudaStream_t stream) {
   KvStoreArgs p{};
   p.key = a.key;
@@ -208,6 +218,32 @@ void launch_kv_store(const KvPrefillArgs &a, cudaStream_t stream) {
   } else {
     a.activations_f32 ? launch(kv_store_kernel<true, false>) : launch(kv_store_kernel<false, false>);
   }
+}
+
+} // namespace
+
+// The rows into the cache (and into the workspace, for what attention does not read as it lies there), then attention.
+void launch_kv_prefill(const KvPrefillArgs &a, cudaStream_t stream) {
+  const KvVisible seen = kv_visible(a.tokens, a.past, a.window, a.sinks);
+  PrefillArgs args{};
+  args.query = a.query;
+  args.key = a.key;
+  args.value = a.value;
+  args.gate = a.gate;
+  args.output = a.output;
+  args.kv_cache = a.caches.single;
+  args.tokens = a.tokens;
+  args.past_tokens = a.past;
+  args.max_context_tokens = a.caches.single_rows;
+  args.query_heads = a.query_heads;
+  args.kv_heads = a.caches.kv_heads;
+  args.activations_f32 = a.activations_f32;
+  args.window = PrefillWindow{a.window, a.sinks, seen.low, seen.sinks, a.workspace,
+                              static_cast<std::uint32_t>(kv_staged_rows(seen, a.past + a.tokens))};
+  if (a.workspace != nullptr) {
+    launch_kv_store(a, stream);
+  }
+  launch_prefill_attention(args, stream);
 }
 
 } // namespace rib200

@@ -153,6 +153,39 @@ struct PrefillParams {
   unsigned int *status;
 };
 
+// Windowed form: a query at position q sees keys [0, min(sinks, low)) and [low, q], low = max(0, q + 1 - window).  A tile walks
+// the key blocks of the first kind that any of its rows sees, then those of the second kind; a block may come in both.
+// Every load is clipped to rows that some query of the launch sees: the maps of the second kind start at token `origin`, the
+// first query's low, and those of the first kind end behind the last sink, so that blocks read zeros for what lies outside.
+struct WindowForm {
+  CUtensorMap k_sink_map;
+  CUtensorMap v_sink_map;
+  std::uint32_t window;
+  std::uint32_t sinks;
+  std::uint32_t origin;
+  std::uint32_t staged; // the maps lead to a copy that holds the chunk's own rows, too
+};
+struct NoWindow {};
+template <bool Window> using WindowOf = std::conditional_t<Window, WindowForm, NoWindow>;
+
+// Key blocks of a tile whose first query is at position `first` and whose last one is at `last`.
+struct TileBlocks {
+  std::uint32_t sinks;  // of the first kind, from block 0 on
+  std::uint32_t window; // first block of the second kind
+  std::uint32_t end;    // one behind the last
+  __host__ __device__ std::uint32_t count() const { return sinks + end - window; }
+  __host__ __device__ std::uint32_t block(std::uint32_t index) const {
+    return index < sinks ? index : window + (index - sinks);
+  }
+};
+__host__ __device__ inline TileBlocks tile_blocks_of(std::uint32_t first, std::uint32_t last, std::uint32_t window,
+                                                     std::uint32_t sinks) {
+  const std::uint32_t low_first = first + 1 > window ? first + 1 - window : 0U;
+  const std::uint32_t low_last = last + 1 > window ? last + 1 - window : 0U;
+  return TileBlocks{((sinks < low_last ? sinks : low_last) + kBlockKeys - 1) / kBlockKeys, low_first / kBlockKeys,
+                    last / kBlockKeys + 1};
+}
+
 __device__ __forceinline__ std::uint32_t smem_u32(const void *p) {
   return static_cast<std::uint32_t>(__cvta_generic_to_shared(p));
 }
@@ -575,11 +608,12 @@ template <> struct Exchange<1> {
   static constexpr int kLanding = 0;
 };
 
-template <bool F32, bool Pair, int Parts>
+template <bool F32, bool Pair, int Parts, bool Window>
 __global__ void __launch_bounds__(kThreads, 1)
     prefill_attention_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
                              const __grid_constant__ CUtensorMap v_map, const __grid_constant__ CUtensorMap k_new_map,
-                             const __grid_constant__ CUtensorMap v_new_map, const PrefillParams p) {
+                             const __grid_constant__ CUtensorMap v_new_map, const PrefillParams p,
+                             const __grid_constant__ WindowOf<Window> w) {
   extern __shared__ __align__(1024) unsigned char smem[];
   const std::uint32_t base = smem_u32(smem); // the 128-byte swizzle needs 1 KiB alignment; checked below
   const std::uint32_t q_smem = base;
@@ -678,8 +712,24 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto tile_rows = [&](std::uint32_t tile) {
     return min(static_cast<std::uint32_t>(kTileRows), p.tokens - tile * kTileRows);
   };
-  auto tile_blocks = [&](std::uint32_t tile) {
+  auto tile_end = [&](std::uint32_t tile) {
     return (p.past + tile * kTileRows + tile_rows(tile) - 1) / kBlockKeys + 1; // newest visible key / 128 + 1
+  };
+  // windowed form: which blocks a tile walks
+  [[maybe_unused]] auto window_blocks = [&](std::uint32_t tile) {
+    if constexpr (Window) {
+      const std::uint32_t first = p.past + tile * kTileRows;
+      return tile_blocks_of(first, first + tile_rows(tile) - 1, w.window, w.sinks);
+    } else {
+      return TileBlocks{0, 0, tile_end(tile)};
+    }
+  };
+  auto tile_blocks = [&](std::uint32_t tile) {
+    if constexpr (Window) {
+      return window_blocks(tile).count();
+    } else {
+      return tile_end(tile);
+    }
   };
   // bytes of a message: only the tile's live rows travel
   [[maybe_unused]] auto message_bytes = [&](std::uint32_t tile) {
@@ -731,7 +781,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool is_value = (entry >> 30) & 1U;
         const std::uint32_t half = (entry >> 29) & 1U;
         const int kv = static_cast<int>((entry >> 16) & 0xFFU);
-        const int key0 = static_cast<int>((entry & 0xFFFFU) * kBlockKeys);
+        int key0 = static_cast<int>((entry & 0xFFFFU) * kBlockKeys);
+        if constexpr (Window) {
+          key0 -= static_cast<int>(w.origin);
+        }
         const std::uint32_t src = ring + slot * kSlotBytes;
         if constexpr (Pair) {
           if (is_value) {
@@ -765,8 +818,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const std::uint32_t head = Pair ? walk.head() * 2 + rank : walk.head();
         const std::uint32_t kv_head = head / p.group;
         const std::uint32_t row0 = walk.tile() * kTileRows;
-        const std::uint32_t all_blocks = tile_blocks(walk.tile());
+        const std::uint32_t all_blocks = tile_end(walk.tile());
         const std::uint32_t block0 = first_block(walk.tile()); // this CTA walks blocks block0 .. block0 + blocks - 1
+        [[maybe_unused]] const TileBlocks walked = window_blocks(walk.tile()); // (windowed: of this list)
         const std::uint32_t blocks = my_blocks(walk.tile());
         if (Split && blocks == 0) {
           continue; // the item is left to the first half of the cluster
@@ -820,7 +874,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         // K travels as two slots per block split by head dims (128 keys x 128 dims each, so that one MMA spans
         // all 128 keys); V as two slots split by keys (64 keys x 256 dims each).
         const bool appends = !F32 && head % p.group == (Pair ? rank : 0U); // serves the group's first head
-        auto load_half = [&](bool is_value, std::uint32_t block, std::uint32_t half) {
+        auto load_half = [&](bool is_value, std::uint32_t index, std::uint32_t half) {
+          const std::uint32_t block = Window ? walked.block(index) : index;
+          const bool is_sink = Window && index < walked.sinks;
           const std::uint32_t slot = n % kSlots;
           if (n >= kSlots) {
             if (!mbar_wait(bar(kBarEmpty + slot), ((n / kSlots) - 1) & 1U, abort_flag)) {
@@ -831,14 +887,24 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
           const std::uint32_t dst = ring + slot * kSlotBytes;
-          const bool from_inputs = !F32 && block * kBlockKeys >= p.past;
+          bool from_inputs = !F32 && block * kBlockKeys >= p.past;
+          if constexpr (Window) {
+            from_inputs = from_inputs && w.staged == 0;
+          }
           if (!from_inputs && (block + 1) * kBlockKeys > p.past) {
             wait_for_append();
           }
           const CUtensorMap *k_src = from_inputs ? &k_new_map : &k_map;
           const CUtensorMap *v_src = from_inputs ? &v_new_map : &v_map;
-          const int block_key0 = static_cast<int>(block * kBlockKeys - (from_inputs ? p.past : 0U));
-          if (appends && from_inputs && block + 1 == all_blocks) {
+          int block_key0 = static_cast<int>(block * kBlockKeys - (from_inputs ? p.past : 0U));
+          if constexpr (Window) {
+            if (!from_inputs) {
+              k_src = is_sink ? &w.k_sink_map : &k_map;
+              v_src = is_sink ? &w.v_sink_map : &v_map;
+              block_key0 = static_cast<int>(block * kBlockKeys) - static_cast<int>(is_sink ? 0U : w.origin);
+            }
+          }
+          if (appends && from_inputs && !is_sink && block + 1 == all_blocks) {
             pending[slot] = 0x80000000U | (is_value ? 0x40000000U : 0U) | (half << 29) | (kv_head << 16) | block;
           }
           if constexpr (Pair) {
@@ -1091,6 +1157,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         continue;
       }
       const std::uint32_t q_pos = p.past + row0 + row; // position of this row's query (rows past the tile are idle)
+      [[maybe_unused]] const TileBlocks walked = window_blocks(walk.tile());
 
       float m_used = -INFINITY; // maximum the exponentials are taken against (scaled, base 2); same in both groups
       float l_sum = 0.0F;       // this thread's share of the row sum
@@ -1124,8 +1191,27 @@ __global__ void __launch_bounds__(kThreads, 1)
           x[e] = __uint_as_float(xr[e >> 5][e & 31]);
         }
         // causal mask: key position j*128 + c is visible iff <= q_pos (also hides rows the context never held)
-        const std::uint32_t key0 = (block0 + j) * kBlockKeys;
-        if (key0 + kBlockKeys - 1 > p.past + row0) {
+        const std::uint32_t key0 = (Window ? walked.block(block0 + j) : block0 + j) * kBlockKeys;
+        if constexpr (Window) {
+          const bool is_sink = block0 + j < walked.sinks;
+          auto low_of = [&](std::uint32_t position) { return position + 1 > w.window ? position + 1 - w.window : 0U; };
+          const std::uint32_t first_pos = p.past + row0;
+          const bool whole = is_sink ? key0 + kBlockKeys <= min(w.sinks, low_of(first_pos))
+                                     : key0 + kBlockKeys - 1 <= first_pos && key0 >= low_of(first_pos + rows - 1);
+          if (!whole) {
+            // visible are the keys [from, to)
+            const std::uint32_t low = low_of(q_pos);
+            const int mine0 = static_cast<int>(key0 + group * 64);
+            const int from = static_cast<int>(is_sink ? 0U : low) - mine0;
+            const int to = static_cast<int>(is_sink ? min(w.sinks, low) : q_pos + 1) - mine0;
+#pragma unroll
+            for (int e = 0; e < 64; ++e) {
+              if (e < from || e >= to) {
+                x[e] = -INFINITY;
+              }
+            }
+          }
+        } else if (key0 + kBlockKeys - 1 > p.past + row0) {
           const int visible = static_cast<int>(q_pos) - static_cast<int>(key0 + group * 64) + 1;
 #pragma unroll
           for (int e = 0; e < 64; ++e) {
@@ -1446,8 +1532,10 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int h = 0; h < 8; ++h) {
                 const float g0f = __uint_as_float(gw[h] << 16);
                 const float g1f = __uint_as_float(gw[h] & 0xFFFF0000U);
-                const float r0 = __uint_as_float(v[e + 2 * h]) * inv * sigmoid_for_bf16(g0f);
-                const float r1 = __uint_as_float(v[e + 2 * h + 1]) * inv * sigmoid_for_bf16(g1f);
+                // (the windowed form keeps small gates' relative precision)
+                const float r0 = __uint_as_float(v[e + 2 * h]) * inv * (Window ? fast_sigmoid(g0f) : sigmoid_for_bf16(g0f));
+                const float r1 =
+                    __uint_as_float(v[e + 2 * h + 1]) * inv * (Window ? fast_sigmoid(g1f) : sigmoid_for_bf16(g1f));
                 ow[h] = pack_bf16(r0, r1);
               }
               st_global_v8(static_cast<__nv_bfloat16 *>(p.output) + dst_base + c * 32 + e, ow);
@@ -1563,15 +1651,23 @@ CUtensorMap make_map(void *base, int rank, const cuuint64_t *dims, const cuuint6
   return map;
 }
 
+// Key blocks that a tile of the launch walks.
+std::uint32_t blocks_of_tile(const PrefillArgs &a, std::uint32_t tile) {
+  const std::uint32_t first = a.past_tokens + tile * kTileRows;
+  const std::uint32_t last = a.past_tokens + std::min<std::uint32_t>(a.tokens, (tile + 1) * kTileRows) - 1;
+  return a.window.window == 0 ? last / kBlockKeys + 1
+                              : tile_blocks_of(first, last, a.window.window, a.window.sinks).count();
+}
+
 // Returns the number of clusters of the split form that fit the device at once (0 for the other forms).
-template <bool F32, bool Pair, int Parts> int configure_once() {
+template <bool F32, bool Pair, int Parts, bool Window> int configure_once() {
   static std::once_flag flags[64];
   static int clusters[64] = {};
   int device = 0;
   cuda_ok(cudaGetDevice(&device), "cudaGetDevice");
   require(device >= 0 && device < 64, "device ordinal out of range", RIB200_STATUS_INTERNAL);
   std::call_once(flags[device], [&] {
-    cuda_ok(cudaFuncSetAttribute(prefill_attention_kernel<F32, Pair, Parts>,
+    cuda_ok(cudaFuncSetAttribute(prefill_attention_kernel<F32, Pair, Parts, Window>,
                                  cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  kSmemBytes),
             "prefill attention shared-memory opt-in");
@@ -1587,7 +1683,7 @@ template <bool F32, bool Pair, int Parts> int configure_once() {
       config.dynamicSmemBytes = kSmemBytes;
       config.attrs = &shape;
       config.numAttrs = 1;
-      cuda_ok(cudaOccupancyMaxActiveClusters(&clusters[device], prefill_attention_kernel<F32, Pair, Parts>, &config),
+      cuda_ok(cudaOccupancyMaxActiveClusters(&clusters[device], prefill_attention_kernel<F32, Pair, Parts, Window>, &config),
               "prefill attention cluster count");
     }
   });
@@ -1617,19 +1713,21 @@ constexpr bool pair_form_enabled() { return true; }
 constexpr bool split_form_enabled() { return true; }
 #endif
 
-template <bool F32, bool Pair, int Parts> void launch(const PrefillArgs &a, cudaStream_t stream) {
-  (void)configure_once<F32, Pair, Parts>();
+template <bool F32, bool Pair, int Parts, bool Window> void launch(const PrefillArgs &a, cudaStream_t stream) {
+  (void)configure_once<F32, Pair, Parts, Window>();
   auto *cache = static_cast<__nv_bfloat16 *>(a.kv_cache);
   // The attention kernel itself writes the key blocks that lie wholly inside this chunk into the cache (BF16
   // inputs).  The append kernel covers the rest: every row for FP32 inputs, else the chunk's rows that share a key
   // block with the past.
   const std::uint32_t ragged = a.past_tokens % kBlockKeys == 0 ? 0U : kBlockKeys - a.past_tokens % kBlockKeys;
-  const std::uint32_t append_rows = F32 ? a.tokens : std::min<std::uint32_t>(a.tokens, ragged);
+  // (A staged context holds all of the chunk's rows already; what is left to do for FP32 are the queries.)
+  const bool staged = Window && a.window.staged != nullptr;
+  const std::uint32_t append_rows = staged ? 0U : F32 ? a.tokens : std::min<std::uint32_t>(a.tokens, ragged);
   // where this GPU's output tiles go (the head-sharded form writes into a wider buffer at a head offset)
   void *own_output = a.output_count == 0 ? a.output : a.outputs[a.output_self];
   const std::uint32_t out_heads = a.output_count == 0 ? a.query_heads : a.output_heads;
   const std::uint32_t out_head_offset = a.output_count == 0 ? 0U : a.output_head_offset;
-  if (append_rows > 0) {
+  if (append_rows > 0 || (staged && F32)) {
     const std::size_t kv_pieces = static_cast<std::size_t>(append_rows) * a.kv_heads * 32 * 2;
     const std::size_t q_pieces = F32 ? static_cast<std::size_t>(a.tokens) * a.query_heads * 32 : 0; // parked queries
     launch_programmatic(prefill_append_kernel<F32>, dim3(static_cast<unsigned int>((kv_pieces + q_pieces + 255) / 256)),
@@ -1642,18 +1740,36 @@ template <bool F32, bool Pair, int Parts> void launch(const PrefillArgs &a, cuda
   // K / V: [kv head][row < context][256], rows 512 bytes apart, heads max_ctx rows apart.  The single-CTA form
   // loads K in boxes of 128 keys and V in boxes of 64; the pair form the other way round (each CTA takes 64 keys
   // of K and all 128 keys of half of V's dims).
-  const cuuint64_t kv_dims[3] = {kHeadDim, context, a.kv_heads};
-  const cuuint64_t kv_strides[2] = {kHeadDim * 2, static_cast<cuuint64_t>(a.max_context_tokens) * kHeadDim * 2};
+  // Windowed form: of the context, what the launch's queries see, in the cache or in the staged copy.
+  const std::uint32_t origin = Window ? a.window.low : 0U;
+  const std::uint32_t plane_rows = staged ? a.window.staged_rows : a.max_context_tokens;
+  auto *rows = staged ? static_cast<__nv_bfloat16 *>(a.window.staged) : cache;
+  auto *window_rows = rows + static_cast<std::size_t>(staged ? a.window.seen_sinks : origin) * kHeadDim;
+  const std::size_t plane = static_cast<std::size_t>(a.kv_heads) * plane_rows * kHeadDim;
+  const cuuint64_t kv_dims[3] = {kHeadDim, context - origin, a.kv_heads};
+  const cuuint64_t kv_strides[2] = {kHeadDim * 2, static_cast<cuuint64_t>(plane_rows) * kHeadDim * 2};
   const cuuint32_t tall_box[3] = {kBoxCols, kBlockKeys, 1};
   const cuuint32_t short_box[3] = {kBoxCols, kHalfKeys, 1};
-  const CUtensorMap k_map = make_map(cache, 3, kv_dims, kv_strides, Pair ? short_box : tall_box);
-  const CUtensorMap v_map =
-      make_map(cache + static_cast<std::size_t>(a.kv_heads) * a.max_context_tokens * kHeadDim, 3, kv_dims, kv_strides,
-               Pair ? tall_box : short_box);
+  const CUtensorMap k_map = make_map(window_rows, 3, kv_dims, kv_strides, Pair ? short_box : tall_box);
+  const CUtensorMap v_map = make_map(window_rows + plane, 3, kv_dims, kv_strides, Pair ? tall_box : short_box);
+  WindowOf<Window> form{};
+  if constexpr (Window) {
+    form.window = a.window.window;
+    form.sinks = a.window.sinks;
+    form.origin = origin;
+    form.staged = staged ? 1U : 0U;
+    form.k_sink_map = k_map;
+    form.v_sink_map = v_map;
+    if (a.window.seen_sinks > 0) {
+      const cuuint64_t sink_dims[3] = {kHeadDim, a.window.seen_sinks, a.kv_heads};
+      form.k_sink_map = make_map(rows, 3, sink_dims, kv_strides, Pair ? short_box : tall_box);
+      form.v_sink_map = make_map(rows + plane, 3, sink_dims, kv_strides, Pair ? tall_box : short_box);
+    }
+  }
   // BF16 key / value inputs, [token][kv head][256]: the same boxes over this chunk's own rows
   CUtensorMap k_new_map = k_map;
   CUtensorMap v_new_map = v_map;
-  if (!F32) {
+  if (!F32 && !staged) {
     const cuuint64_t new_dims[3] = {kHeadDim, a.tokens, a.kv_heads};
     const cuuint64_t new_strides[2] = {static_cast<cuuint64_t>(a.kv_heads) * kHeadDim * 2, kHeadDim * 2};
     k_new_map = make_map(const_cast<void *>(a.key), 3, new_dims, new_strides, Pair ? short_box : tall_box);
@@ -1699,12 +1815,11 @@ template <bool F32, bool Pair, int Parts> void launch(const PrefillArgs &a, cuda
   params.group = a.query_heads / a.kv_heads;
   {
     // every item when already the first tile is long enough to be worth a hand-over, else only the long ones
-    const std::uint32_t first_tile_blocks =
-        (a.past_tokens + std::min<std::uint32_t>(a.tokens, kTileRows) - 1) / kBlockKeys + 1;
+    const std::uint32_t first_tile_blocks = blocks_of_tile(a, 0);
     params.split_min_blocks = first_tile_blocks >= kSplitMinBlocks ? kSplitMinBlocks : kSplitMinBlocksLate;
   }
   params.status = device_status_word();
-  params.wait_first = append_rows == 0 ? 1U : 0U;
+  params.wait_first = append_rows == 0 && !(staged && F32) ? 1U : 0U;
 
   cudaLaunchConfig_t config{};
   int device = 0;
@@ -1733,7 +1848,7 @@ template <bool F32, bool Pair, int Parts> void launch(const PrefillArgs &a, cuda
   attributes[1].val.clusterDim.z = 1;
   config.attrs = attributes;
   config.numAttrs = Pair || Parts > 1 ? 2 : 1;
-  cuda_ok(cudaLaunchKernelEx(&config, prefill_attention_kernel<F32, Pair, Parts>, q_map, k_map, v_map, k_new_map, v_new_map, params),
+  cuda_ok(cudaLaunchKernelEx(&config, prefill_attention_kernel<F32, Pair, Parts, Window>, q_map, k_map, v_map, k_new_map, v_new_map, params, form),
           "prefill attention launch");
 }
 
@@ -1757,11 +1872,10 @@ void launch_prefill_attention(const PrefillArgs &args, cudaStream_t stream) {
   cuda_ok(cudaGetDevice(&device), "cudaGetDevice");
   cuda_ok(cudaDeviceGetAttribute(&sm_count, cudaDevAttrMultiProcessorCount, device), "SM count query");
   const std::uint32_t tiles = (args.tokens + kTileRows - 1) / kTileRows;
-  const std::uint32_t first_tile_blocks =
-      (args.past_tokens + std::min<std::uint32_t>(args.tokens, kTileRows) - 1) / kBlockKeys + 1;
+  const std::uint32_t first_tile_blocks = blocks_of_tile(args, 0);
   // ... or few items of which only the late ones are long (a rank's slice of the heads of a long prompt): those are
   // split, the short ones are left to one CTA (or pair) of their cluster.
-  const std::uint32_t last_tile_blocks = (args.past_tokens + args.tokens - 1) / kBlockKeys + 1;
+  const std::uint32_t last_tile_blocks = blocks_of_tile(args, tiles - 1);
   const bool split = split_form_enabled() && 2 * tiles * args.query_heads <= static_cast<std::uint32_t>(sm_count) &&
                      (first_tile_blocks >= kSplitMinBlocks || last_tile_blocks >= kSplitMinBlocksLate);
   // ... and between four where that still leaves half of the GPU free (one tile of the model's heads) and gives each two
@@ -1770,33 +1884,42 @@ void launch_prefill_attention(const PrefillArgs &args, cudaStream_t stream) {
                         8 * tiles * args.query_heads <= static_cast<std::uint32_t>(sm_count) &&
                         first_tile_blocks >= kQuarterMinBlocks;
   const bool pair = pair_form_enabled() && (args.query_heads / args.kv_heads) % 2 == 0;
-  auto dispatch = [&](auto f32) {
+  auto dispatch = [&](auto f32, auto windowed) {
     constexpr bool kF32 = decltype(f32)::value;
+    constexpr bool kWindow = decltype(windowed)::value;
     // clusters of the quarter form that the device holds at once
     auto quarters_fit = [&] {
-      const std::uint32_t fit = static_cast<std::uint32_t>(pair ? configure_once<kF32, true, 4>() : configure_once<kF32, false, 4>());
+      const std::uint32_t fit = static_cast<std::uint32_t>(pair ? configure_once<kF32, true, 4, kWindow>()
+                                                                : configure_once<kF32, false, 4, kWindow>());
       return tiles * args.query_heads / (pair ? 2 : 1) <= fit;
     };
     if (quarters && quarters_fit()) {
       if (pair) {
-        launch<kF32, true, 4>(args, stream);
+        launch<kF32, true, 4, kWindow>(args, stream);
       } else {
-        launch<kF32, false, 4>(args, stream);
+        launch<kF32, false, 4, kWindow>(args, stream);
       }
     } else if (split && pair) {
-      launch<kF32, true, 2>(args, stream);
+      launch<kF32, true, 2, kWindow>(args, stream);
     } else if (split) {
-      launch<kF32, false, 2>(args, stream);
+      launch<kF32, false, 2, kWindow>(args, stream);
     } else if (pair) {
-      launch<kF32, true, 1>(args, stream);
+      launch<kF32, true, 1, kWindow>(args, stream);
     } else {
-      launch<kF32, false, 1>(args, stream);
+      launch<kF32, false, 1, kWindow>(args, stream);
     }
   };
-  if (args.activations_f32) {
-    dispatch(std::true_type{});
+  auto dispatch_type = [&](auto windowed) {
+    if (args.activations_f32) {
+      dispatch(std::true_type{}, windowed);
+    } else {
+      dispatch(std::false_type{}, windowed);
+    }
+  };
+  if (args.window.window != 0) {
+    dispatch_type(std::true_type{});
   } else {
-    dispatch(std::false_type{});
+    dispatch_type(std::false_type{});
   }
 }
 

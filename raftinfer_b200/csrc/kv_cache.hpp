@@ -140,22 +140,15 @@ __device__ __forceinline__ KvView kv_view(const KvCaches &c, std::uint32_t seque
   v.eight_bit = c.eight_bit;
   return v;
 }
-__device__ __forceinline__ std::uint32_t kv_capacity(const KvCaches &c, std::uint32_t sequence) {
-  return c.tables != nullptr ? c.max_blocks * kKvPageTokens
-                             : c.caches != nullptr ? c.capacities[sequence] : c.single_rows;
-}
-// Whether sequence's token at `pos` can be served; else the status bits that say why not (none for padding).
-__device__ __forceinline__ bool kv_servable(const KvCaches &c, std::uint32_t sequence, std::uint32_t pos, std::uint32_t &why) {
-  why = 0;
-  if (pos == RIB200_NO_POSITION) {
-    return false;
-  }
-  if (pos >= kv_capacity(c, sequence)) {
-    why = RIB200_DEVICE_POSITION_OUT_OF_RANGE;
-  } else if (c.caches != nullptr && reinterpret_cast<std::uintptr_t>(c.caches[sequence]) % 16 != 0) {
-    why = RIB200_DEVICE_POINTER_MISALIGNED; // the pointers lie in device memory: the host cannot see them
-  }
-  return why == 0;
+// Why a sequence's token at `pos` cannot be served: status bits, kKvPadding for an entry that is to be skipped, or 0.
+constexpr std::uint32_t kKvPadding = 1U << 31;
+__device__ __forceinline__ std::uint32_t kv_refusal(const KvCaches &c, const KvView &view, std::uint32_t pos) {
+  const std::uint32_t capacity = c.tables != nullptr ? c.max_blocks * kKvPageTokens : view.rows;
+  std::uint32_t why = 0;
+  // the pointers lie in device memory: the host cannot see them
+  why = reinterpret_cast<std::uintptr_t>(view.base) % 16 != 0 ? RIB200_DEVICE_POINTER_MISALIGNED : why;
+  why = pos >= capacity ? RIB200_DEVICE_POSITION_OUT_OF_RANGE : why;
+  return pos == RIB200_NO_POSITION ? kKvPadding : why;
 }
 #endif
 

@@ -76,119 +76,126 @@ struct DecodeParams {
   float *parts; // [2 * kMaxCtas][kPartFloats]
   unsigned int *status;
   std::uint32_t group;
-  std::uint32_t ctas; // of the first kernel
+  std::uint32_t ctas;      // of the first kernel
+  std::uint32_t min_steps; // of a piece
 };
 
-// ---- schedule: the same arithmetic in both kernels ----
+// ---- schedule: the same arithmetic in both kernels, by every warp for itself (no barrier, no shared memory) ----
 struct Row { // what one sequence's query sees
   std::uint32_t pos, low, sinks; // tokens [0, sinks) and [low, pos]
   std::uint32_t sink_steps, window_step; // steps [0, sink_steps), then from window_step on
   std::uint32_t steps;
+  KvView view;
 };
 
 __device__ __forceinline__ Row row_of(const KvDecodeArgs &a, std::uint32_t sequence, std::uint32_t &why) {
-  Row r{};
+  Row r;
   r.pos = a.positions[sequence];
-  if (!kv_servable(a.caches, sequence, r.pos, why)) {
-    return r;
-  }
+  r.view = kv_view(a.caches, sequence);
+  why = kv_refusal(a.caches, r.view, r.pos);
   r.low = r.pos + 1 > a.window ? r.pos + 1 - a.window : 0U;
   r.sinks = min(a.sinks, r.low);
   r.window_step = r.low / kStep;
   r.sink_steps = min((r.sinks + kStep - 1) / kStep, r.window_step);
-  r.steps = r.sink_steps + (r.pos / kStep - r.window_step + 1);
+  r.steps = why == 0 ? r.sink_steps + (r.pos / kStep - r.window_step + 1) : 0U;
   return r;
 }
 
 using Count = unsigned long long;
 
-// exclusive prefix over the block's threads, and the total; `sums` holds an entry for each warp
-__device__ __forceinline__ Count scan(Count v, Count *sums, Count &total) {
-  const std::uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, warps = blockDim.x / 32;
+// exclusive prefix over the lanes, and the total
+__device__ __forceinline__ Count scan(Count v, Count &total) {
   Count inclusive = v;
 #pragma unroll
   for (int step = 1; step < 32; step *= 2) {
     const Count below = __shfl_up_sync(0xFFFFFFFFU, inclusive, step);
-    inclusive += lane >= static_cast<std::uint32_t>(step) ? below : 0;
+    inclusive += threadIdx.x % 32 >= static_cast<std::uint32_t>(step) ? below : 0;
   }
-  __syncthreads(); // `sums` is free
-  if (lane == 31) {
-    sums[warp] = inclusive;
-  }
-  __syncthreads();
-  Count before = 0;
-  total = 0;
-  for (std::uint32_t w = 0; w < warps; ++w) {
-    before += w < warp ? sums[w] : 0;
-    total += sums[w];
-  }
-  return before + inclusive - v;
+  total = __shfl_sync(0xFFFFFFFFU, inclusive, 31);
+  return inclusive - v;
 }
 
 struct Schedule {
   std::uint32_t target; // steps of a piece where rows are cut by themselves, else 0
   Count units;          // pieces or, laid end to end, steps
   std::uint32_t pieces; // CTAs with work
+  Count each;           // units / pieces, and the remainder
+  std::uint32_t more;
   // the unit that was asked for
   std::uint32_t sequence, head, index;
+  // first unit of piece i
+  __device__ __forceinline__ Count bound(std::uint32_t i) const { return each * i + min(i, more); }
 };
-__device__ __forceinline__ Count unit_bound(const Schedule &s, std::uint32_t piece) { return s.units * piece / s.pieces; }
 
-// Finds the schedule, and where unit `of(schedule)` lies.  Called by the whole block.
-template <int MinSteps, class Of> __device__ __forceinline__ Schedule make_schedule(const DecodeParams &p, bool report, Of of) {
-  __shared__ Count sums[8];
-  __shared__ std::uint32_t found[3];
+// Finds the schedule, and where unit `of(schedule)` lies.  A lane looks at a run of neighbouring sequences.
+template <class Of> __device__ __forceinline__ Schedule make_schedule(const DecodeParams &p, bool report, Of of) {
+  const std::uint32_t lane = threadIdx.x % 32;
   const std::uint32_t heads = p.a.caches.kv_heads;
-  const std::uint32_t share = (p.a.batch + blockDim.x - 1) / blockDim.x;
-  const std::uint32_t first = min(p.a.batch, threadIdx.x * share), last = min(p.a.batch, first + share);
+  const std::uint32_t share = (p.a.batch + 31) / 32;
+  const std::uint32_t first = min(p.a.batch, lane * share), last = min(p.a.batch, first + share);
   Count mine = 0;
   std::uint32_t why_all = 0;
+  std::uint32_t only = 0; // steps of the lane's one sequence where it has no more
+#pragma unroll 4
   for (std::uint32_t i = first; i < last; ++i) {
     std::uint32_t why;
-    mine += row_of(p.a, i, why).steps;
+    only = row_of(p.a, i, why).steps;
+    mine += only;
     why_all |= why;
   }
+  why_all &= ~kKvPadding;
   if (report && why_all != 0) {
     atomicOr(p.status, why_all);
   }
-  Schedule s{};
+  Schedule s;
   Count total;
-  Count before = scan(mine, sums, total) * heads;
+  Count before = scan(mine, total) * heads;
+  s.target = 0;
   s.units = total * heads;
   const std::uint32_t rows = p.a.batch * heads;
+  auto units_of = [&](std::uint32_t i) {
+    std::uint32_t steps = only;
+    if (share > 1) {
+      std::uint32_t why;
+      steps = row_of(p.a, i, why).steps;
+    }
+    return s.target != 0 ? (steps + s.target - 1) / s.target : steps;
+  };
   if (2 * rows <= p.ctas) {
-    const Count room = p.ctas - rows;
-    s.target = static_cast<std::uint32_t>(max(static_cast<Count>(MinSteps), (s.units + room - 1) / room));
+    const std::uint32_t room = p.ctas - rows;
+    s.target = static_cast<std::uint32_t>(max(static_cast<Count>(p.min_steps), (s.units + room - 1) / room));
     mine = 0;
     for (std::uint32_t i = first; i < last; ++i) {
-      std::uint32_t why;
-      mine += (row_of(p.a, i, why).steps + s.target - 1) / s.target;
+      mine += units_of(i);
     }
-    before = scan(mine, sums, total) * heads;
+    before = scan(mine, total) * heads;
     s.units = total * heads;
     s.pieces = static_cast<std::uint32_t>(s.units);
   } else {
-    s.pieces = static_cast<std::uint32_t>(min(static_cast<Count>(p.ctas), (s.units + MinSteps - 1) / MinSteps));
+    s.pieces = static_cast<std::uint32_t>(min(static_cast<Count>(p.ctas), (s.units + p.min_steps - 1) / p.min_steps));
   }
+  s.each = s.pieces != 0 ? s.units / s.pieces : 0;
+  s.more = static_cast<std::uint32_t>(s.units - s.each * s.pieces);
   const Count unit = of(s);
-  Count at = before;
-  for (std::uint32_t i = first; i < last && unit < s.units; ++i) {
-    std::uint32_t why;
-    std::uint32_t each = row_of(p.a, i, why).steps;
-    if (s.target != 0) {
-      each = (each + s.target - 1) / s.target;
+  bool found = false;
+  std::uint32_t at_sequence = 0, at_head = 0, at_index = 0;
+  for (std::uint32_t i = first; i < last && unit >= before && !found; ++i) {
+    const std::uint32_t each = units_of(i);
+    const Count end = before + static_cast<Count>(each) * heads;
+    if (unit < end) {
+      const std::uint32_t into = static_cast<std::uint32_t>(unit - before); // below 2^31 steps a head ...
+      at_sequence = i;
+      at_head = static_cast<std::uint32_t>((unit - before) / each);
+      at_index = into - at_head * each;                                     // ... so that wrapping leaves this right
+      found = true;
     }
-    if (unit >= at && unit < at + static_cast<Count>(each) * heads) {
-      found[0] = i;
-      found[1] = static_cast<std::uint32_t>((unit - at) / each);
-      found[2] = static_cast<std::uint32_t>((unit - at) % each);
-    }
-    at += static_cast<Count>(each) * heads;
+    before = end;
   }
-  __syncthreads();
-  s.sequence = found[0];
-  s.head = found[1];
-  s.index = found[2];
+  const std::uint32_t who = __ballot_sync(0xFFFFFFFFU, found);
+  const int from = who != 0 ? __ffs(who) - 1 : 0;
+  s.sequence = __shfl_sync(0xFFFFFFFFU, at_sequence, from);
+  s.head = __shfl_sync(0xFFFFFFFFU, at_head, from);
+  s.index = __shfl_sync(0xFFFFFFFFU, at_index, from);
   return s;
 }
 
@@ -420,6 +427,95 @@ template <bool F32, bool EightBit> struct Query {
   }
 };
 
+// A lane's eight dims of the new token's row, fetched when its piece begins.
+template <bool F32> struct NewRow {
+  uint4 raw[F32 ? 2 : 1];
+  __device__ __forceinline__ void load(const void *base, std::size_t index) {
+    const uint4 *at = reinterpret_cast<const uint4 *>(static_cast<const unsigned char *>(base) + index * (F32 ? 4 : 2));
+    raw[0] = at[0];
+    if constexpr (F32) {
+      raw[1] = at[1];
+    }
+  }
+  __device__ __forceinline__ void get(float (&x)[8]) const {
+    const std::uint32_t w[4] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (F32) {
+        x[i] = __uint_as_float(w[i]);
+      } else {
+        x[2 * i] = __uint_as_float(w[i] << 16);
+        x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000U);
+      }
+    }
+    if constexpr (F32) {
+      x[4] = __uint_as_float(raw[1].x);
+      x[5] = __uint_as_float(raw[1].y);
+      x[6] = __uint_as_float(raw[1].z);
+      x[7] = __uint_as_float(raw[1].w);
+    }
+  }
+};
+
+// The new token's row into the cache and into its slot, which holds the rows of its block: row r of the block whose first row
+// is row r0 of the plane.  Not inlined: one step in many comes here.
+template <bool EightBit>
+__device__ __noinline__ void append_row(std::uint32_t slot, unsigned char *plane, std::uint32_t r0, std::uint32_t r, float x0,
+                                        float x1, float x2, float x3, float x4, float x5, float x6, float x7) {
+  using L = Slot<EightBit>;
+  const std::uint32_t lane = threadIdx.x % 32;
+  const float x[8] = {x0, x1, x2, x3, x4, x5, x6, x7};
+  if constexpr (EightBit) {
+    unsigned char *record = plane + static_cast<std::size_t>(r0 / kStep) * kKv8BlockBytes;
+    float amax = 0.0F;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      amax = fmaxf(amax, kv8_finite_magnitude(x[e]));
+    }
+#pragma unroll
+    for (int step = 16; step > 0; step /= 2) {
+      amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFU, amax, step));
+    }
+    const float before = r > 0 ? lds_float(slot + kSlotScale) : 0.0F;
+    const float scale = fmaxf(kv8_scale(amax), before);
+    const float inverse = kv8_inverse(scale);
+    __syncwarp(); // everyone has the scale in front
+    if (lane == 0) {
+      sts_float(slot + kSlotScale, scale);
+      *reinterpret_cast<float *>(record + kKv8CodeBytes) = scale;
+    }
+    if (scale != before) {
+      const float ratio = before * inverse;
+#pragma unroll 1
+      for (std::uint32_t i = 0; i < r; ++i) {
+        const uint2 old = lds64(slot + L::row(i) + 8 * lane);
+        std::uint32_t w[2] = {old.x, old.y};
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float2 a = kv8_values2(w[k] & 0xFFFFU), b = kv8_values2(w[k] >> 16);
+          w[k] = kv8_codes2(a.x * ratio, a.y * ratio) | (kv8_codes2(b.x * ratio, b.y * ratio) << 16);
+        }
+        sts64(slot + L::row(i) + 8 * lane, make_uint2(w[0], w[1]));
+        *reinterpret_cast<uint2 *>(record + i * kKvHeadDim + 8 * lane) = make_uint2(w[0], w[1]);
+      }
+    }
+    std::uint32_t w[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      w[k] = kv8_codes2(x[4 * k] * inverse, x[4 * k + 1] * inverse) |
+             (kv8_codes2(x[4 * k + 2] * inverse, x[4 * k + 3] * inverse) << 16);
+    }
+    sts64(slot + L::row(r) + 8 * lane, make_uint2(w[0], w[1]));
+    *reinterpret_cast<uint2 *>(record + r * kKvHeadDim + 8 * lane) = make_uint2(w[0], w[1]);
+  } else {
+    const uint4 raw = make_uint4(split2<false>(x[0], x[1], 0), split2<false>(x[2], x[3], 0), split2<false>(x[4], x[5], 0),
+                                 split2<false>(x[6], x[7], 0));
+    sts128(slot + L::row(r) + 16 * lane, raw);
+    *reinterpret_cast<uint4 *>(plane + static_cast<std::size_t>(r0 + r) * 512 + 16 * lane) = raw;
+  }
+  __syncwarp();
+}
+
 template <bool F32, bool EightBit>
 __global__ void __launch_bounds__(Shape<EightBit>::kWarps * 32, Shape<EightBit>::kCtasPerSm)
     kv_decode_kernel(const __grid_constant__ DecodeParams p) {
@@ -443,8 +539,8 @@ __global__ void __launch_bounds__(Shape<EightBit>::kWarps * 32, Shape<EightBit>:
   grid_dependency_wait();
   grid_dependents_may_launch();
 
-  const Schedule plan = make_schedule<static_cast<int>(kWarps)>(p, blockIdx.x == 0, [](const Schedule &s) {
-    return s.target != 0 ? static_cast<Count>(blockIdx.x) : blockIdx.x < s.pieces ? unit_bound(s, blockIdx.x) : s.units;
+  const Schedule plan = make_schedule(p, blockIdx.x == 0 && warp == 0, [](const Schedule &s) {
+    return s.target != 0 ? static_cast<Count>(blockIdx.x) : blockIdx.x < s.pieces ? s.bound(blockIdx.x) : s.units;
   });
   if (blockIdx.x >= plan.pieces) {
     return;
@@ -453,7 +549,7 @@ __global__ void __launch_bounds__(Shape<EightBit>::kWarps * 32, Shape<EightBit>:
   std::uint32_t sequence = plan.sequence;
   std::uint32_t head = plan.head;
   std::uint32_t step = plan.target != 0 ? plan.index * plan.target : plan.index;
-  Count left = plan.target != 0 ? plan.target : unit_bound(plan, blockIdx.x + 1) - unit_bound(plan, blockIdx.x);
+  Count left = plan.target != 0 ? plan.target : plan.bound(blockIdx.x + 1) - plan.bound(blockIdx.x);
   bool first_row = true;
   std::uint32_t used = 0;    // slots of this warp in the rows so far
   std::uint32_t issued = 0;  // ... that have been asked for
@@ -466,7 +562,7 @@ __global__ void __launch_bounds__(Shape<EightBit>::kWarps * 32, Shape<EightBit>:
     const std::uint32_t begin = step;
     const std::uint32_t end = static_cast<std::uint32_t>(min(static_cast<Count>(row.steps), begin + left));
     left -= end - begin;
-    const KvView view = kv_view(p.a.caches, sequence);
+    const KvView &view = row.view;
     const std::uint32_t my_steps = end - begin > warp ? (end - begin - warp + kWarps - 1) / kWarps : 0;
     const std::uint32_t my_slots = 2 * my_steps;
     auto token_of = [&](std::uint32_t s) { return (s < row.sink_steps ? s : row.window_step + (s - row.sink_steps)) * kStep; };
@@ -537,65 +633,22 @@ __global__ void __launch_bounds__(Shape<EightBit>::kWarps * 32, Shape<EightBit>:
         (static_cast<std::size_t>(sequence) * p.a.query_heads + head * p.group) * kKvHeadDim;
     q.load(p.a.query, q_base, p.group, g, t);
 
-    // The new token's row into the cache and into its slot (which holds the rows of its block); `is_value` 1: the V row.
+    // The new token's row belongs to the row's last step.
+    const bool appends = end == row.steps && my_steps != 0 && (end - 1 - begin) % kWarps == warp;
+    NewRow<F32> fresh[2];
+    if (appends) {
+      const std::size_t index =
+          (static_cast<std::size_t>(sequence) * p.a.caches.kv_heads + head) * kKvHeadDim + 8 * lane;
+      fresh[0].load(p.a.key, index);
+      fresh[1].load(p.a.value, index);
+    }
     auto append = [&](std::uint32_t slot, std::uint32_t is_value, std::uint32_t tok0) {
       unsigned char *plane = view.plane(is_value, head, tok0);
-      if (plane == nullptr) {
-        return;
+      if (plane != nullptr) {
+        float x[8];
+        fresh[is_value].get(x);
+        append_row<EightBit>(slot, plane, view.row_in_plane(tok0), row.pos - tok0, x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]);
       }
-      const std::uint32_t r = row.pos - tok0;
-      const std::uint32_t r0 = view.row_in_plane(tok0);
-      float x[8];
-      load8<F32>(is_value != 0 ? p.a.value : p.a.key,
-                 (static_cast<std::size_t>(sequence) * p.a.caches.kv_heads + head) * kKvHeadDim + 8 * lane, x);
-      if constexpr (EightBit) {
-        unsigned char *record = plane + static_cast<std::size_t>(r0 / kStep) * kKv8BlockBytes;
-        float amax = 0.0F;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          amax = fmaxf(amax, kv8_finite_magnitude(x[e]));
-        }
-#pragma unroll
-        for (int step_ = 16; step_ > 0; step_ /= 2) {
-          amax = fmaxf(amax, __shfl_xor_sync(0xFFFFFFFFU, amax, step_));
-        }
-        const float before = r > 0 ? lds_float(slot + kSlotScale) : 0.0F;
-        const float scale = fmaxf(kv8_scale(amax), before);
-        const float inverse = kv8_inverse(scale);
-        __syncwarp(); // everyone has the scale in front
-        if (lane == 0) {
-          sts_float(slot + kSlotScale, scale);
-          *reinterpret_cast<float *>(record + kKv8CodeBytes) = scale;
-        }
-        if (scale != before) {
-          const float ratio = before * inverse;
-          for (std::uint32_t i = 0; i < r; ++i) {
-            const uint2 old = lds64(slot + L::row(i) + 8 * lane);
-            std::uint32_t w[2] = {old.x, old.y};
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const float2 a = kv8_values2(w[k] & 0xFFFFU), b = kv8_values2(w[k] >> 16);
-              w[k] = kv8_codes2(a.x * ratio, a.y * ratio) | (kv8_codes2(b.x * ratio, b.y * ratio) << 16);
-            }
-            sts64(slot + L::row(i) + 8 * lane, make_uint2(w[0], w[1]));
-            *reinterpret_cast<uint2 *>(record + i * kKvHeadDim + 8 * lane) = make_uint2(w[0], w[1]);
-          }
-        }
-        std::uint32_t w[2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          w[k] = kv8_codes2(x[4 * k] * inverse, x[4 * k + 1] * inverse) |
-                 (kv8_codes2(x[4 * k + 2] * inverse, x[4 * k + 3] * inverse) << 16);
-        }
-        sts64(slot + L::row(r) + 8 * lane, make_uint2(w[0], w[1]));
-        *reinterpret_cast<uint2 *>(record + r * kKvHeadDim + 8 * lane) = make_uint2(w[0], w[1]);
-      } else {
-        const uint4 raw = make_uint4(split2<false>(x[0], x[1], 0), split2<false>(x[2], x[3], 0),
-                                     split2<false>(x[4], x[5], 0), split2<false>(x[6], x[7], 0));
-        sts128(slot + L::row(r) + 16 * lane, raw);
-        *reinterpret_cast<uint4 *>(plane + static_cast<std::size_t>(r0 + r) * 512 + 16 * lane) = raw;
-      }
-      __syncwarp();
     };
 
     float oacc[16][4];
@@ -609,7 +662,7 @@ __global__ void __launch_bounds__(Shape<EightBit>::kWarps * 32, Shape<EightBit>:
 
     for (std::uint32_t i = 0; i < my_steps; ++i) {
       const std::uint32_t tok0 = token_of(begin + warp + i * kWarps);
-      const bool newest = row.pos - tok0 < kStep;
+      const bool newest = appends && i + 1 == my_steps;
       const bool whole = tok0 + kStep <= row.pos + 1 && (tok0 >= row.low || tok0 + kStep <= row.sinks);
       auto seen = [&](std::uint32_t token) { return token <= row.pos && (token >= row.low || token < row.sinks); };
 
@@ -795,6 +848,17 @@ __global__ void __launch_bounds__(Shape<EightBit>::kWarps * 32, Shape<EightBit>:
     run_sum += __shfl_xor_sync(0xFFFFFFFFU, run_sum, 16);
 
     // ---- the warps' shares of this row's part come together ----
+    const bool alone = begin == 0 && end == row.steps;
+    float4 gate[2]; // of this thread's items
+    if (alone) {
+#pragma unroll
+      for (std::uint32_t i = 0; i < 2; ++i) {
+        const std::uint32_t item = threadIdx.x + i * kWarps * 32;
+        if (item < p.group * 64) {
+          gate[i] = load4<F32>(p.a.gate, q_base + item / 64 * kKvHeadDim + item % 64 * 4);
+        }
+      }
+    }
     const bool stop = __syncthreads_or(!healthy ? 1 : 0) != 0; // every warp has left its ring: the merge area lies there
     float *merge = reinterpret_cast<float *>(smem);
     float *warp_max = merge;                      // [warp][head]
@@ -823,10 +887,15 @@ __global__ void __launch_bounds__(Shape<EightBit>::kWarps * 32, Shape<EightBit>:
       }
     }
     __syncthreads();
-    const bool alone = begin == 0 && end == row.steps;
     float *part = p.parts + static_cast<std::size_t>(plan.target != 0 ? blockIdx.x : 2 * blockIdx.x + (first_row ? 0 : 1)) *
                                 kPartFloats;
-    for (std::uint32_t item = threadIdx.x; item < p.group * 64; item += kWarps * 32) {
+    static_assert(2 * kWarps * 32 >= kGroup * 64, "two items a thread at most");
+#pragma unroll
+    for (std::uint32_t i = 0; i < 2; ++i) {
+      const std::uint32_t item = threadIdx.x + i * kWarps * 32;
+      if (item >= p.group * 64) {
+        break;
+      }
       const std::uint32_t h = item / 64;
       const std::uint32_t dim0 = item % 64 * 4;
       float top = warp_max[h];
@@ -847,7 +916,7 @@ __global__ void __launch_bounds__(Shape<EightBit>::kWarps * 32, Shape<EightBit>:
       out = make_float4(out.x * inverse, out.y * inverse, out.z * inverse, out.w * inverse);
       if (alone) {
         const std::size_t index = q_base + h * kKvHeadDim + dim0;
-        store4<F32>(p.a.output, index, gated(out, load4<F32>(p.a.gate, index)));
+        store4<F32>(p.a.output, index, gated(out, gate[i]));
       } else {
         *reinterpret_cast<float4 *>(part + h * kKvHeadDim + dim0) = out;
         if (dim0 == 0) {
@@ -875,15 +944,16 @@ __global__ void __launch_bounds__(Shape<EightBit>::kWarps * 32, Shape<EightBit>:
 
 // Puts the parts of a row together.  grid = (rows that may be shared, query heads of a KV head); four groups of 64 threads take
 // the parts in turn, a thread four dims.
-template <bool F32> __global__ void __launch_bounds__(256) kv_combine_kernel(const __grid_constant__ DecodeParams p, int min_steps) {
+template <bool F32> __global__ void __launch_bounds__(256) kv_combine_kernel(const __grid_constant__ DecodeParams p) {
   __shared__ float group_max[4], group_sum[4];
   __shared__ float4 group_out[4][64];
   grid_dependents_may_launch();
-  grid_dependency_wait();
-  auto unit = [](const Schedule &s) { // the first of a row's own pieces, or the last step in front of a cut
-    return s.target != 0 ? static_cast<Count>(blockIdx.x) : blockIdx.x + 1 < s.pieces ? unit_bound(s, blockIdx.x + 1) - 1 : s.units;
-  };
-  const Schedule plan = min_steps == 4 ? make_schedule<4>(p, false, unit) : make_schedule<8>(p, false, unit);
+  // The first kernel lets this one in when everything in front of both has ended: positions, tables and gates are there, and
+  // only the parts have to be waited for.
+  const Schedule plan = make_schedule(p, false, [](const Schedule &s) {
+    // the first of a row's own pieces, or the last step in front of a cut
+    return s.target != 0 ? static_cast<Count>(blockIdx.x) : blockIdx.x + 1 < s.pieces ? s.bound(blockIdx.x + 1) - 1 : s.units;
+  });
   if (blockIdx.x >= plan.pieces) {
     return;
   }
@@ -905,17 +975,17 @@ template <bool F32> __global__ void __launch_bounds__(256) kv_combine_kernel(con
       return;
     }
     const Row row = row_of(p.a, plan.sequence, why);
-    const Count cut = unit_bound(plan, blockIdx.x + 1);
+    const Count cut = plan.bound(blockIdx.x + 1);
     const Count row_begin = cut - 1 - plan.index;
     const Count row_end = row_begin + row.steps;
-    const Count piece_begin = unit_bound(plan, blockIdx.x);
+    const Count piece_begin = plan.bound(blockIdx.x);
     if (cut >= row_end || (piece_begin > row_begin)) {
       return;
     }
     first = blockIdx.x;
     // pieces first .. the one with the row's last step
     std::uint32_t last = first + 1;
-    while (unit_bound(plan, last + 1) < row_end) {
+    while (plan.bound(last + 1) < row_end) {
       ++last;
     }
     count = last - first + 1;
@@ -924,6 +994,13 @@ template <bool F32> __global__ void __launch_bounds__(256) kv_combine_kernel(con
   }
   const std::uint32_t h = blockIdx.y;
   const std::uint32_t lane = threadIdx.x % 64, group = threadIdx.x / 64;
+  const std::size_t index =
+      (static_cast<std::size_t>(plan.sequence) * p.a.query_heads + plan.head * p.group + h) * kKvHeadDim + lane * 4;
+  float4 gate = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
+  if (group == 0) {
+    gate = load4<F32>(p.a.gate, index);
+  }
+  grid_dependency_wait();
   auto slot = [&](std::uint32_t i) {
     return p.parts + static_cast<std::size_t>(i == 0 ? first_slot : (first + i) * stride) * kPartFloats;
   };
@@ -975,11 +1052,9 @@ template <bool F32> __global__ void __launch_bounds__(256) kv_combine_kernel(con
       y.z += group_out[i][lane].z * weight;
       y.w += group_out[i][lane].w * weight;
     }
-    const std::size_t index =
-        (static_cast<std::size_t>(plan.sequence) * p.a.query_heads + plan.head * p.group + h) * kKvHeadDim + lane * 4;
     const float inverse = 1.0F / total;
     y = make_float4(y.x * inverse, y.y * inverse, y.z * inverse, y.w * inverse);
-    store4<F32>(p.a.output, index, gated(y, load4<F32>(p.a.gate, index)));
+    store4<F32>(p.a.output, index, gated(y, gate));
   }
 }
 
@@ -1002,10 +1077,10 @@ template <bool F32, bool EightBit> void launch(DecodeParams p, cudaStream_t stre
   cuda_ok(cudaGetDevice(&device), "cudaGetDevice");
   cuda_ok(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device), "SM count query");
   p.ctas = std::min<std::uint32_t>(kMaxCtas, static_cast<std::uint32_t>(sms * S::kCtasPerSm));
+  p.min_steps = S::kWarps;
   launch_programmatic(kv_decode_kernel<F32, EightBit>, dim3(p.ctas), dim3(S::kWarps * 32), S::kSmemBytes, stream,
                       "KV decode launch", p);
-  launch_programmatic(kv_combine_kernel<F32>, dim3(p.ctas, p.group), dim3(256), 0, stream, "KV decode combine launch", p,
-                      S::kWarps);
+  launch_programmatic(kv_combine_kernel<F32>, dim3(p.ctas, p.group), dim3(256), 0, stream, "KV decode combine launch", p);
 }
 
 } // namespace

@@ -78,6 +78,7 @@ struct DecodeParams {
   std::uint32_t group;
   std::uint32_t ctas;      // of the first kernel
   std::uint32_t min_steps; // of a piece
+  std::uint32_t by_rows;   // rows are cut by themselves
 };
 
 // ---- schedule: the same arithmetic in both kernels, by every warp for itself (no barrier, no shared memory) ----
@@ -121,54 +122,56 @@ struct Schedule {
   std::uint32_t pieces; // CTAs with work
   Count each;           // units / pieces, and the remainder
   std::uint32_t more;
-  // the unit that was asked for
-  std::uint32_t sequence, head, index;
+  // the lane's run of neighbouring sequences, the units in front of it, and the steps of its sequence if it has only one
+  std::uint32_t first, last, share, only;
+  Count before;
+
   // first unit of piece i
   __device__ __forceinline__ Count bound(std::uint32_t i) const { return each * i + min(i, more); }
+  // units of one of the lane's sequences, for each head
+  __device__ __forceinline__ std::uint32_t units_of(const DecodeParams &p, std::uint32_t sequence) const {
+    std::uint32_t steps = only;
+    if (share > 1) {
+      std::uint32_t why;
+      steps = row_of(p.a, sequence, why).steps;
+    }
+    return target != 0 ? (steps + target - 1) / target : steps;
+  }
 };
 
-// Finds the schedule, and where unit `of(schedule)` lies.  A lane looks at a run of neighbouring sequences.
-template <class Of> __device__ __forceinline__ Schedule make_schedule(const DecodeParams &p, bool report, Of of) {
+__device__ __forceinline__ Schedule make_schedule(const DecodeParams &p, bool report) {
   const std::uint32_t lane = threadIdx.x % 32;
   const std::uint32_t heads = p.a.caches.kv_heads;
-  const std::uint32_t share = (p.a.batch + 31) / 32;
-  const std::uint32_t first = min(p.a.batch, lane * share), last = min(p.a.batch, first + share);
+  Schedule s;
+  s.share = (p.a.batch + 31) / 32;
+  s.first = min(p.a.batch, lane * s.share);
+  s.last = min(p.a.batch, s.first + s.share);
+  s.target = 0;
+  s.only = 0;
   Count mine = 0;
   std::uint32_t why_all = 0;
-  std::uint32_t only = 0; // steps of the lane's one sequence where it has no more
 #pragma unroll 4
-  for (std::uint32_t i = first; i < last; ++i) {
+  for (std::uint32_t i = s.first; i < s.last; ++i) {
     std::uint32_t why;
-    only = row_of(p.a, i, why).steps;
-    mine += only;
+    s.only = row_of(p.a, i, why).steps;
+    mine += s.only;
     why_all |= why;
   }
   why_all &= ~kKvPadding;
   if (report && why_all != 0) {
     atomicOr(p.status, why_all);
   }
-  Schedule s;
   Count total;
-  Count before = scan(mine, total) * heads;
-  s.target = 0;
+  s.before = scan(mine, total) * heads;
   s.units = total * heads;
-  const std::uint32_t rows = p.a.batch * heads;
-  auto units_of = [&](std::uint32_t i) {
-    std::uint32_t steps = only;
-    if (share > 1) {
-      std::uint32_t why;
-      steps = row_of(p.a, i, why).steps;
-    }
-    return s.target != 0 ? (steps + s.target - 1) / s.target : steps;
-  };
-  if (2 * rows <= p.ctas) {
-    const std::uint32_t room = p.ctas - rows;
+  if (p.by_rows != 0) {
+    const std::uint32_t room = p.ctas - p.a.batch * heads;
     s.target = static_cast<std::uint32_t>(max(static_cast<Count>(p.min_steps), (s.units + room - 1) / room));
     mine = 0;
-    for (std::uint32_t i = first; i < last; ++i) {
-      mine += units_of(i);
+    for (std::uint32_t i = s.first; i < s.last; ++i) {
+      mine += s.units_of(p, i);
     }
-    before = scan(mine, total) * heads;
+    s.before = scan(mine, total) * heads;
     s.units = total * heads;
     s.pieces = static_cast<std::uint32_t>(s.units);
   } else {
@@ -176,27 +179,48 @@ template <class Of> __device__ __forceinline__ Schedule make_schedule(const Deco
   }
   s.each = s.pieces != 0 ? s.units / s.pieces : 0;
   s.more = static_cast<std::uint32_t>(s.units - s.each * s.pieces);
-  const Count unit = of(s);
+  return s;
+}
+
+struct Place {
+  std::uint32_t sequence, head, index; // the index-th unit of a row
+};
+// Where a unit lies.
+__device__ __forceinline__ Place place_of(const Schedule &s, const DecodeParams &p, Count unit) {
+  Place at{};
   bool found = false;
-  std::uint32_t at_sequence = 0, at_head = 0, at_index = 0;
-  for (std::uint32_t i = first; i < last && unit >= before && !found; ++i) {
-    const std::uint32_t each = units_of(i);
-    const Count end = before + static_cast<Count>(each) * heads;
+  Count before = s.before;
+  for (std::uint32_t i = s.first; i < s.last && unit >= before && !found; ++i) {
+    const std::uint32_t each = s.units_of(p, i);
+    const Count end = before + static_cast<Count>(each) * p.a.caches.kv_heads;
     if (unit < end) {
-      const std::uint32_t into = static_cast<std::uint32_t>(unit - before); // below 2^31 steps a head ...
-      at_sequence = i;
-      at_head = static_cast<std::uint32_t>((unit - before) / each);
-      at_index = into - at_head * each;                                     // ... so that wrapping leaves this right
+      at.sequence = i;
+      at.head = static_cast<std::uint32_t>((unit - before) / each);
+      // a row has less than 2^31 units, so that wrapping leaves this right
+      at.index = static_cast<std::uint32_t>(unit - before) - at.head * each;
       found = true;
     }
     before = end;
   }
   const std::uint32_t who = __ballot_sync(0xFFFFFFFFU, found);
   const int from = who != 0 ? __ffs(who) - 1 : 0;
-  s.sequence = __shfl_sync(0xFFFFFFFFU, at_sequence, from);
-  s.head = __shfl_sync(0xFFFFFFFFU, at_head, from);
-  s.index = __shfl_sync(0xFFFFFFFFU, at_index, from);
-  return s;
+  at.sequence = __shfl_sync(0xFFFFFFFFU, at.sequence, from);
+  at.head = __shfl_sync(0xFFFFFFFFU, at.head, from);
+  at.index = __shfl_sync(0xFFFFFFFFU, at.index, from);
+  return at;
+}
+// Units of a row and the first of them.
+__device__ __forceinline__ std::uint32_t units_of_row(const Schedule &s, const DecodeParams &p, std::uint32_t sequence,
+                                                      std::uint32_t head, Count &first) {
+  Count at = s.before;
+  std::uint32_t each = 0;
+  for (std::uint32_t i = s.first; i < s.last && i <= sequence; ++i) {
+    each = s.units_of(p, i);
+    at += i < sequence ? static_cast<Count>(each) * p.a.caches.kv_heads : static_cast<Count>(each) * head;
+  }
+  const int from = static_cast<int>(sequence / s.share);
+  first = __shfl_sync(0xFFFFFFFFU, at, from);
+  return __shfl_sync(0xFFFFFFFFU, each, from);
 }
 
 // ---- small pieces ----
@@ -539,16 +563,15 @@ __global__ void __launch_bounds__(Shape<EightBit>::kWarps * 32, Shape<EightBit>:
   grid_dependency_wait();
   grid_dependents_may_launch();
 
-  const Schedule plan = make_schedule(p, blockIdx.x == 0 && warp == 0, [](const Schedule &s) {
-    return s.target != 0 ? static_cast<Count>(blockIdx.x) : blockIdx.x < s.pieces ? s.bound(blockIdx.x) : s.units;
-  });
+  const Schedule plan = make_schedule(p, blockIdx.x == 0 && warp == 0);
   if (blockIdx.x >= plan.pieces) {
     return;
   }
+  const Place start = place_of(plan, p, plan.target != 0 ? static_cast<Count>(blockIdx.x) : plan.bound(blockIdx.x));
   const std::uint64_t policy = evict_first_policy();
-  std::uint32_t sequence = plan.sequence;
-  std::uint32_t head = plan.head;
-  std::uint32_t step = plan.target != 0 ? plan.index * plan.target : plan.index;
+  std::uint32_t sequence = start.sequence;
+  std::uint32_t head = start.head;
+  std::uint32_t step = plan.target != 0 ? start.index * plan.target : start.index;
   Count left = plan.target != 0 ? plan.target : plan.bound(blockIdx.x + 1) - plan.bound(blockIdx.x);
   bool first_row = true;
   std::uint32_t used = 0;    // slots of this warp in the rows so far
@@ -942,78 +965,83 @@ __global__ void __launch_bounds__(Shape<EightBit>::kWarps * 32, Shape<EightBit>:
   }
 }
 
-// Puts the parts of a row together.  grid = (rows that may be shared, query heads of a KV head); four groups of 64 threads take
-// the parts in turn, a thread four dims.
-template <bool F32> __global__ void __launch_bounds__(256) kv_combine_kernel(const __grid_constant__ DecodeParams p) {
-  __shared__ float group_max[4], group_sum[4];
-  __shared__ float4 group_out[4][64];
+// Puts the parts of a row together.  Where rows are cut by themselves there are few rows and many parts: grid = (rows, query
+// heads of a KV head), eight groups of 64 threads take the parts in turn.  Else there are many rows of two or three parts: a
+// block for every cut between two CTAs, which serves the row that the cut is the first one in, 64 threads a query head.  A
+// thread has four dims.
+constexpr std::uint32_t kCombineGroups = 8;
+template <bool F32>
+__global__ void __launch_bounds__(kCombineGroups * 64) kv_combine_kernel(const __grid_constant__ DecodeParams p) {
+  __shared__ float group_max[kCombineGroups], group_sum[kCombineGroups];
+  __shared__ float4 group_out[kCombineGroups][64];
   grid_dependents_may_launch();
   // The first kernel lets this one in when everything in front of both has ended: positions, tables and gates are there, and
   // only the parts have to be waited for.
-  const Schedule plan = make_schedule(p, false, [](const Schedule &s) {
-    // the first of a row's own pieces, or the last step in front of a cut
-    return s.target != 0 ? static_cast<Count>(blockIdx.x) : blockIdx.x + 1 < s.pieces ? s.bound(blockIdx.x + 1) - 1 : s.units;
-  });
-  if (blockIdx.x >= plan.pieces) {
-    return;
-  }
-  std::uint32_t why;
-  std::uint32_t first, count; // parts
-  std::uint32_t stride, first_slot;
-  if (plan.target != 0) {
-    const Row row = row_of(p.a, plan.sequence, why);
-    first = blockIdx.x;
-    count = (row.steps + plan.target - 1) / plan.target;
-    if (plan.index != 0 || count == 1) {
+  const std::uint32_t lane = threadIdx.x % 64;
+  // What is queued behind this kernel may rely on the first one having ended: one block at least stays until it has.
+  auto leave = [] {
+    if (blockIdx.x == 0 && blockIdx.y == 0) {
+      grid_dependency_wait();
+    }
+  };
+  const Schedule plan = make_schedule(p, false);
+  Place row;
+  std::uint32_t count, first, first_slot;
+  if (p.by_rows != 0) {
+    row.sequence = blockIdx.x / p.a.caches.kv_heads;
+    row.head = blockIdx.x % p.a.caches.kv_heads;
+    Count unit;
+    count = units_of_row(plan, p, row.sequence, row.head, unit);
+    first = first_slot = static_cast<std::uint32_t>(unit);
+    if (count <= 1) {
+      leave();
       return;
     }
-    first_slot = first;
-    stride = 1;
   } else {
-    // cut c = blockIdx.x + 1 lies at step `cut`; it is this block's row if it is the first cut inside a row
     if (blockIdx.x + 1 >= plan.pieces) {
+      leave();
       return;
     }
-    const Row row = row_of(p.a, plan.sequence, why);
-    const Count cut = plan.bound(blockIdx.x + 1);
-    const Count row_begin = cut - 1 - plan.index;
-    const Count row_end = row_begin + row.steps;
-    const Count piece_begin = plan.bound(blockIdx.x);
-    if (cut >= row_end || (piece_begin > row_begin)) {
-      return;
+    const Count piece_begin = plan.bound(blockIdx.x), cut = plan.bound(blockIdx.x + 1);
+    row = place_of(plan, p, cut - 1);
+    std::uint32_t why;
+    const Count row_begin = cut - 1 - row.index;
+    const Count row_end = row_begin + row_of(p.a, row.sequence, why).steps;
+    if (cut >= row_end || piece_begin > row_begin) {
+      leave();
+      return; // no cut inside a row, or not the first one
     }
     first = blockIdx.x;
-    // pieces first .. the one with the row's last step
-    std::uint32_t last = first + 1;
+    std::uint32_t last = first + 1; // the piece with the row's last step
     while (plan.bound(last + 1) < row_end) {
       ++last;
     }
     count = last - first + 1;
     first_slot = 2 * first + (piece_begin == row_begin ? 0U : 1U);
-    stride = 2;
   }
-  const std::uint32_t h = blockIdx.y;
-  const std::uint32_t lane = threadIdx.x % 64, group = threadIdx.x / 64;
+  const std::uint32_t h = p.by_rows != 0 ? blockIdx.y : threadIdx.x / 64;
+  const std::uint32_t group = p.by_rows != 0 ? threadIdx.x / 64 : 0;
+  const std::uint32_t groups = p.by_rows != 0 ? kCombineGroups : 1;
   const std::size_t index =
-      (static_cast<std::size_t>(plan.sequence) * p.a.query_heads + plan.head * p.group + h) * kKvHeadDim + lane * 4;
+      (static_cast<std::size_t>(row.sequence) * p.a.query_heads + row.head * p.group + h) * kKvHeadDim + lane * 4;
   float4 gate = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
   if (group == 0) {
     gate = load4<F32>(p.a.gate, index);
   }
   grid_dependency_wait();
   auto slot = [&](std::uint32_t i) {
-    return p.parts + static_cast<std::size_t>(i == 0 ? first_slot : (first + i) * stride) * kPartFloats;
+    return p.parts + static_cast<std::size_t>(i == 0 ? first_slot : (first + i) * (p.by_rows != 0 ? 1U : 2U)) * kPartFloats;
   };
   float top = kLowest, sum = 0.0F;
   float4 out = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
   constexpr std::uint32_t kAtOnce = 8;
-  for (std::uint32_t i = group; i < count; i += 4 * kAtOnce) {
+  for (std::uint32_t i = group; i < count; i += groups * kAtOnce) {
     float m[kAtOnce], l[kAtOnce];
     float4 v[kAtOnce];
 #pragma unroll
     for (std::uint32_t j = 0; j < kAtOnce; ++j) {
-      if (i + 4 * j < count) {
-        const float *part = slot(i + 4 * j);
+      if (i + groups * j < count) {
+        const float *part = slot(i + groups * j);
         m[j] = part[kGroup * kKvHeadDim + h];
         l[j] = part[kGroup * kKvHeadDim + kGroup + h];
         v[j] = *reinterpret_cast<const float4 *>(part + h * kKvHeadDim + lane * 4);
@@ -1021,7 +1049,7 @@ template <bool F32> __global__ void __launch_bounds__(256) kv_combine_kernel(con
     }
 #pragma unroll
     for (std::uint32_t j = 0; j < kAtOnce; ++j) {
-      if (i + 4 * j < count) {
+      if (i + groups * j < count) {
         const float next = fmaxf(top, m[j]);
         const float keep = fast_exp2(top - next), take = l[j] * fast_exp2(m[j] - next);
         sum = sum * keep + take;
@@ -1033,29 +1061,35 @@ template <bool F32> __global__ void __launch_bounds__(256) kv_combine_kernel(con
       }
     }
   }
-  if (lane == 0) {
-    group_max[group] = top;
-    group_sum[group] = sum;
-  }
-  group_out[group][lane] = out;
-  __syncthreads();
-  if (group == 0) {
-    float all = fmaxf(fmaxf(group_max[0], group_max[1]), fmaxf(group_max[2], group_max[3]));
-    float total = 0.0F;
-    float4 y = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float weight = fast_exp2(group_max[i] - all);
-      total += group_sum[i] * weight;
-      y.x += group_out[i][lane].x * weight;
-      y.y += group_out[i][lane].y * weight;
-      y.z += group_out[i][lane].z * weight;
-      y.w += group_out[i][lane].w * weight;
+  if (p.by_rows != 0) {
+    if (lane == 0) {
+      group_max[group] = top;
+      group_sum[group] = sum;
     }
-    const float inverse = 1.0F / total;
-    y = make_float4(y.x * inverse, y.y * inverse, y.z * inverse, y.w * inverse);
-    store4<F32>(p.a.output, index, gated(y, gate));
+    group_out[group][lane] = out;
+    __syncthreads();
+    if (group != 0) {
+      return;
+    }
+#pragma unroll
+    for (std::uint32_t i = 1; i < kCombineGroups; ++i) {
+      top = fmaxf(top, group_max[i]);
+    }
+    sum = 0.0F;
+    out = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
+#pragma unroll
+    for (std::uint32_t i = 0; i < kCombineGroups; ++i) {
+      const float weight = fast_exp2(group_max[i] - top);
+      sum += group_sum[i] * weight;
+      out.x += group_out[i][lane].x * weight;
+      out.y += group_out[i][lane].y * weight;
+      out.z += group_out[i][lane].z * weight;
+      out.w += group_out[i][lane].w * weight;
+    }
   }
+  const float inverse = 1.0F / sum;
+  store4<F32>(p.a.output, index,
+              gated(make_float4(out.x * inverse, out.y * inverse, out.z * inverse, out.w * inverse), gate));
 }
 
 template <bool F32, bool EightBit> void configure_once() {
@@ -1078,9 +1112,13 @@ template <bool F32, bool EightBit> void launch(DecodeParams p, cudaStream_t stre
   cuda_ok(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device), "SM count query");
   p.ctas = std::min<std::uint32_t>(kMaxCtas, static_cast<std::uint32_t>(sms * S::kCtasPerSm));
   p.min_steps = S::kWarps;
+  const std::uint32_t rows = p.a.batch * p.a.caches.kv_heads;
+  p.by_rows = 2 * rows <= p.ctas ? 1U : 0U;
   launch_programmatic(kv_decode_kernel<F32, EightBit>, dim3(p.ctas), dim3(S::kWarps * 32), S::kSmemBytes, stream,
                       "KV decode launch", p);
-  launch_programmatic(kv_combine_kernel<F32>, dim3(p.ctas, p.group), dim3(256), 0, stream, "KV decode combine launch", p);
+  const dim3 grid = p.by_rows != 0 ? dim3(rows, p.group) : dim3(p.ctas - 1);
+  launch_programmatic(kv_combine_kernel<F32>, grid, dim3(64 * (p.by_rows != 0 ? kCombineGroups : p.group)), 0, stream,
+                      "KV decode combine launch", p);
 }
 
 } // namespace

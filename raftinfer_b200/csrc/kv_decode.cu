@@ -50,10 +50,12 @@ constexpr float kWeightUnit = 32768.0F;
 // Slots.  BF16: row pairs (1 KiB, one copy) at a pitch of 1040 bytes; the row index m of the matrix instruction stands for
 // token 2 (m % 8) + m / 8, so that the eight rows of an ldmatrix lie in eight different bank groups.  8 bit: groups of four
 // rows (1 KiB, one copy; the block's scale comes with the last) at a pitch of 1056 bytes, read with 16-byte loads in which
-// eight lanes meet eight different bank groups, see below.
+// eight lanes meet eight different bank groups, see below; K and V of a step share a slot, which halves what a step spends on
+// addresses, waits and fences.  (BF16 rows of one and a half steps are as much as fits.)
 template <bool EightBit> struct Slot {
   static constexpr std::uint32_t kPitch = EightBit ? 1056 : 1040;
-  static constexpr std::uint32_t kBytes = EightBit ? 4224 : 8 * 1040;
+  static constexpr std::uint32_t kValues = EightBit ? 4224 : 0; // where the V rows begin
+  static constexpr std::uint32_t kBytes = EightBit ? 2 * 4224 : 8 * 1040;
   static __device__ __forceinline__ std::uint32_t row(std::uint32_t token) {
     return EightBit ? (token >> 2) * kPitch + (token & 3U) * 256U : (token >> 1) * kPitch + (token & 1U) * 512U;
   }
@@ -62,8 +64,9 @@ constexpr std::uint32_t kSlotScale = 3 * 1056 + 1024; // of an 8-bit slot
 constexpr std::uint32_t kMergePitch = kKvHeadDim + 8;
 
 template <bool EightBit> struct Shape {
-  static constexpr int kWarps = EightBit ? 4 : 4;
-  static constexpr int kSlots = EightBit ? 6 : 3;
+  static constexpr int kWarps = 4;
+  static constexpr int kSlots = 3;
+  static constexpr int kHalves = EightBit ? 1 : 2; // slots of a step
   static constexpr int kCtasPerSm = 2;
   static constexpr std::uint32_t kRingBytes = kWarps * kSlots * Slot<EightBit>::kBytes;
   static constexpr std::uint32_t kSmemBytes = kRingBytes + kWarps * kSlots * 8;
@@ -587,16 +590,16 @@ __global__ void __launch_bounds__(Shape<EightBit>::kWarps * 32, Shape<EightBit>:
     left -= end - begin;
     const KvView &view = row.view;
     const std::uint32_t my_steps = end - begin > warp ? (end - begin - warp + kWarps - 1) / kWarps : 0;
-    const std::uint32_t my_slots = 2 * my_steps;
+    const std::uint32_t my_slots = S::kHalves * my_steps;
     auto token_of = [&](std::uint32_t s) { return (s < row.sink_steps ? s : row.window_step + (s - row.sink_steps)) * kStep; };
 
-    // slot n of this row's part: the K rows (n even) or the V rows of the warp's step n / 2
+    // slot n of this row's part.  8 bit: K and V rows of the warp's step n; BF16: the K rows (n even) or V rows of step n / 2
     auto issue = [&](std::uint32_t n) {
-      const std::uint32_t tok0 = token_of(begin + warp + (n >> 1) * kWarps);
+      const std::uint32_t tok0 = token_of(begin + warp + n / S::kHalves * kWarps);
       const std::uint32_t at = (used + n) % kSlots;
       const std::uint32_t slot = ring + at * L::kBytes;
       const std::uint32_t bar = bars + at * 8;
-      const unsigned char *plane = view.plane(n & 1U, head, tok0);
+      const unsigned char *plane = view.plane(n % S::kHalves, head, tok0);
       const std::uint32_t r0 = view.row_in_plane(tok0);
       ++issued;
       fence_proxy_async(); // earlier accesses to this slot are ordered before the copy
@@ -610,12 +613,14 @@ __global__ void __launch_bounds__(Shape<EightBit>::kWarps * 32, Shape<EightBit>:
       }
       if constexpr (EightBit) {
         if (lane == 0) {
-          mbarrier_expect_tx(bar, kKv8BlockBytes);
+          mbarrier_expect_tx(bar, 2 * kKv8BlockBytes);
         }
         __syncwarp();
-        if (lane < 4) {
-          bulk_copy_g2s(slot + lane * L::kPitch, plane + static_cast<std::size_t>(r0 / kStep) * kKv8BlockBytes + lane * 1024,
-                        lane == 3 ? 1040 : 1024, bar, policy);
+        if (lane < 8) {
+          const std::uint32_t piece = lane & 3U;
+          const unsigned char *src = plane + static_cast<std::size_t>(r0 / kStep) * kKv8BlockBytes + piece * 1024 +
+                                     (lane >= 4 ? view.kv_heads * view.plane_bytes() : 0);
+          bulk_copy_g2s(slot + (lane >= 4 ? L::kValues : 0U) + piece * L::kPitch, src, piece == 3 ? 1040 : 1024, bar, policy);
         }
       } else {
         const std::uint32_t rows = min(kStep, row.pos + 1 - tok0);
@@ -692,13 +697,13 @@ __global__ void __launch_bounds__(Shape<EightBit>::kWarps * 32, Shape<EightBit>:
       // ---- K: logits and weights ----
       fence_proxy_async();
       __syncwarp(); // all lanes are done with the slot that is filled next
-      if (2 * i + kSlots - 1 < my_slots) {
-        issue(2 * i + kSlots - 1);
+      if (S::kHalves * i + kSlots - 1 < my_slots) {
+        issue(S::kHalves * i + kSlots - 1);
       }
-      if (!wait(2 * i)) {
+      if (!wait(S::kHalves * i)) {
         break;
       }
-      const std::uint32_t k_slot = ring + (used + 2 * i) % kSlots * L::kBytes;
+      const std::uint32_t k_slot = ring + (used + S::kHalves * i) % kSlots * L::kBytes;
       if (newest) {
         append(k_slot, 0, tok0);
       }
@@ -765,15 +770,17 @@ __global__ void __launch_bounds__(Shape<EightBit>::kWarps * 32, Shape<EightBit>:
       run_sum += weight_a + weight_b;
 
       // ---- V ----
-      fence_proxy_async();
-      __syncwarp();
-      if (2 * i + kSlots < my_slots) {
-        issue(2 * i + kSlots);
+      if constexpr (S::kHalves == 2) {
+        fence_proxy_async();
+        __syncwarp();
+        if (2 * i + kSlots < my_slots) {
+          issue(2 * i + kSlots);
+        }
+        if (!wait(2 * i + 1)) {
+          break;
+        }
       }
-      if (!wait(2 * i + 1)) {
-        break;
-      }
-      const std::uint32_t v_slot = ring + (used + 2 * i + 1) % kSlots * L::kBytes;
+      const std::uint32_t v_slot = S::kHalves == 2 ? ring + (used + 2 * i + 1) % kSlots * L::kBytes : k_slot + L::kValues;
       if (newest) {
         append(v_slot, 1, tok0);
       }
@@ -1113,7 +1120,7 @@ template <bool F32, bool EightBit> void launch(DecodeParams p, cudaStream_t stre
   p.ctas = std::min<std::uint32_t>(kMaxCtas, static_cast<std::uint32_t>(sms * S::kCtasPerSm));
   p.min_steps = S::kWarps;
   const std::uint32_t rows = p.a.batch * p.a.caches.kv_heads;
-  p.by_rows = 2 * rows <= p.ctas ? 1U : 0U;
+  p.by_rows = 8 * rows <= p.ctas ? 1U : 0U;
   launch_programmatic(kv_decode_kernel<F32, EightBit>, dim3(p.ctas), dim3(S::kWarps * 32), S::kSmemBytes, stream,
                       "KV decode launch", p);
   const dim3 grid = p.by_rows != 0 ? dim3(rows, p.group) : dim3(p.ctas - 1);

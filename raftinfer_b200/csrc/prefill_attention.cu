@@ -72,6 +72,7 @@ constexpr int kRingOffset = kQBytes;
 constexpr int kBarrierOffset = kRingOffset + kSlots * kSlotBytes;
 constexpr int kExchangeOffset = kBarrierOffset + 256;     // row maxima / row sums passed between the two softmax groups
 constexpr int kSmemBytes = kExchangeOffset + 2 * 2 * kTileRows * 4;
+constexpr int kGateBars = 192;                            // behind kBarCount barriers and two words: one for each softmax warp
 constexpr int kSoftmaxThreads = 256;                      // two groups of four warps, 64 score columns per thread
 constexpr int kProducerWarp = 8;
 constexpr int kMmaWarp = 9;
@@ -104,6 +105,7 @@ enum : int {
   kBarStoresDone = 12 + 2 * kSlots, // split form: the producer's write-backs to the cache have read their slots
   kBarCount = 13 + 2 * kSlots
 };
+static_assert(kBarCount * 8 + 8 <= kGateBars && kGateBars + kSoftmaxThreads / 32 * 8 <= 256, "barrier area");
 
 // Optional timeline probe (compile with -DRIB200_TRACE): the first CTA of the grid stamps clock64() at the
 // points named below, 16 stamps per key block, into a device array that rib200_debug_read_trace copies out.
@@ -164,6 +166,8 @@ struct WindowForm {
   std::uint32_t sinks;
   std::uint32_t origin;
   std::uint32_t staged; // the maps lead to a copy that holds the chunk's own rows, too
+  CUtensorMap gate_map;   // BF16 gates and outputs, [token][heads * 256], boxes of 32 tokens x 64 dims
+  CUtensorMap output_map;
 };
 struct NoWindow {};
 template <bool Window> using WindowOf = std::conditional_t<Window, WindowForm, NoWindow>;
@@ -332,6 +336,12 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap *map, int c0, int
                "r"(c0), "r"(c1), "r"(c2), "r"(src)
                : "memory");
 }
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, int c0, int c1, std::uint32_t src) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];\n" ::"l"(
+                   reinterpret_cast<std::uint64_t>(map)),
+               "r"(c0), "r"(c1), "r"(src)
+               : "memory");
+}
 __device__ __forceinline__ void tma_store_commit() { asm volatile("cp.async.bulk.commit_group;\n" ::: "memory"); }
 // the stores of this thread have read their shared-memory source
 __device__ __forceinline__ void tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;\n" ::: "memory"); }
@@ -484,6 +494,16 @@ __device__ __forceinline__ float sigmoid_for_bf16(float x) {
   return fmaf(0.5F, t, 0.5F);
 }
 
+// Two of them with one reciprocal: 1 / a = b * (1 / (a b)).  Gates below -40 count as -40 (4e-18), which keeps a b finite.
+__device__ __forceinline__ void fast_sigmoid2(float x, float y, float &sx, float &sy) {
+  const float a = 1.0F + fast_exp2(fmaxf(x, -40.0F) * -1.4426950408889634F);
+  const float b = 1.0F + fast_exp2(fmaxf(y, -40.0F) * -1.4426950408889634F);
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(a * b));
+  sx = b * r;
+  sy = a * r;
+}
+
 // 1 / (1 + e^-x) through ex2 and an approximate reciprocal (relative error ~1e-6, far below BF16 resolution)
 __device__ __forceinline__ float fast_sigmoid(float x) {
   return __fdividef(1.0F, 1.0F + fast_exp2(x * -1.4426950408889634F));
@@ -633,6 +653,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   // the keys, CTAs 2, 3 the pair that takes the second half.
   constexpr bool Split = Parts > 1;
   using Message = Exchange<Parts>;
+  // Windowed form, BF16: gates come to a softmax warp and outputs leave it as TMA boxes of 32 rows x 64 dims in 4 KiB of its own,
+  // which lie where the ring's fifth slot would be.  (A thread has a row; loading and storing rows 32 bytes a lane touched 32
+  // lines an instruction, kept the memory pipe busy for 4-6 k cycles twice a tile, and the MMA warp's barrier polls waited behind
+  // them: 4096 tokens behind a window of 1024 76.4 -> 67.4 us.  Split items have one tile a CTA, where a slot more in the ring
+  // counts for more: 512 tokens behind 16384, window 4096, 37.4 us so and 39.0 with boxes.)
+  constexpr bool kBoxes = Window && !F32 && Parts == 1;
+  constexpr std::uint32_t kSlots = kBoxes ? rib200::kSlots - 1 : rib200::kSlots;
   constexpr bool kCluster = Pair || Split;
   constexpr std::uint32_t kClusterSize = (Pair ? 2U : 1U) * Parts;
   const std::uint32_t cta = kCluster ? cluster_rank() : 0U;
@@ -660,9 +687,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(bar(kBarPeerFree), Split ? (Parts - 1) * kSoftmaxThreads : 1);
     mbar_init(bar(kBarStoresDone), 1);
     mbar_init(bar(kBarOFree), kRowThreads);
-    for (int s = 0; s < kSlots; ++s) {
+    for (std::uint32_t s = 0; s < kSlots; ++s) {
       mbar_init(bar(kBarFull + s), 1);
       mbar_init(bar(kBarEmpty + s), 1);
+    }
+    if constexpr (kBoxes) {
+      for (int s = 0; s < kSoftmaxThreads / 32; ++s) {
+        mbar_init(bars + kGateBars + s * 8U, 1);
+      }
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(bar(kBarSFull + b), 1);
@@ -1145,6 +1177,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     float *exchange = reinterpret_cast<float *>(smem + kExchangeOffset); // [parity][group][row]
     bool ok = *abort_flag == 0;
     std::uint32_t g0 = 0;
+    // (boxes) this warp's area: rows of 128 bytes, 16-byte pieces in the order of the 128-byte swizzle
+    [[maybe_unused]] unsigned char *box_row = smem + kRingOffset + kSlots * kSlotBytes + warp * 4096 + lane * 128;
+    [[maybe_unused]] const std::uint32_t box = smem_u32(box_row) - lane * 128;
+    [[maybe_unused]] const std::uint32_t gate_bar = bars + kGateBars + warp * 8U;
+    [[maybe_unused]] std::uint32_t gate_parity = 0;
+    [[maybe_unused]] bool gates_asked = false;
 
     for (TileWalk walk(p.tiles, Pair ? p.query_heads / 2 : p.query_heads, units, unit); ok && !walk.done(); walk.next()) {
       const std::uint32_t head = Pair ? walk.head() * 2 + rank : walk.head();
@@ -1158,6 +1196,26 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       const std::uint32_t q_pos = p.past + row0 + row; // position of this row's query (rows past the tile are idle)
       [[maybe_unused]] const TileBlocks walked = window_blocks(walk.tile());
+
+      // the pieces of 32 columns (of the group's four) that this CTA writes
+      const int first_piece = Split && split_here ? max(0, static_cast<int>(part) * Message::kPieces - group * 4) : 0;
+      const int end_piece =
+          Split && split_here ? min(4, (static_cast<int>(part) + 1) * Message::kPieces - group * 4) : 4;
+      const bool live = row < rows && first_piece < end_piece;
+      // (boxes) this warp has rows to write; its columns are then the group's 128, in two boxes
+      [[maybe_unused]] const bool boxes = static_cast<std::uint32_t>((warp & 3) * 32) < rows && first_piece < end_piece;
+      [[maybe_unused]] auto fetch_gates = [&](int half) {
+        if constexpr (kBoxes) {
+          gates_asked = boxes;
+          if (boxes && lane == 0) {
+            tma_store_wait_read(); // the outputs that were here have left
+            mbar_expect_tx(gate_bar, 4096);
+            tma_load_2d(box, &w.gate_map, static_cast<int>(head * kHeadDim + group * 128 + half * kBoxCols),
+                        static_cast<int>(row0 + (warp & 3) * 32), gate_bar);
+          }
+        }
+      };
+      fetch_gates(0);
 
       float m_used = -INFINITY; // maximum the exponentials are taken against (scaled, base 2); same in both groups
       float l_sum = 0.0F;       // this thread's share of the row sum
@@ -1310,13 +1368,40 @@ __global__ void __launch_bounds__(kThreads, 1)
       const std::size_t dst_base =
           (static_cast<std::size_t>(row0 + row) * p.output_heads + p.output_head_offset + head) * kHeadDim +
           group * 128;
-      // the pieces of 32 columns (of the group's four) that this CTA writes
-      const int first_piece = Split && split_here ? max(0, static_cast<int>(part) * Message::kPieces - group * 4) : 0;
-      const int end_piece =
-          Split && split_here ? min(4, (static_cast<int>(part) + 1) * Message::kPieces - group * 4) : 4;
-      const bool live = row < rows && first_piece < end_piece;
-      uint4 gate_raw[16]; // BF16 gates of this thread's 128 columns, fetched while the last PV is still running
-      if constexpr (!F32) {
+      // (boxes) the sigmoids of the first 64 columns are made while the last PV is still running; their box is then free for
+      // the gates of the other 64
+      [[maybe_unused]] float gates[kBoxes ? 64 : 1];
+      [[maybe_unused]] auto take_gates = [&] {
+        if constexpr (kBoxes) {
+          if (boxes) {
+            ok = mbar_wait(gate_bar, gate_parity, abort_flag);
+            ok = __all_sync(0xFFFFFFFFU, ok);
+            gate_parity ^= 1U;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const uint4 raw = *reinterpret_cast<const uint4 *>(box_row + ((i ^ (lane & 7)) << 4));
+              const std::uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+              for (int h = 0; h < 4; ++h) {
+                fast_sigmoid2(__uint_as_float(words[h] << 16), __uint_as_float(words[h] & 0xFFFF0000U),
+                              gates[8 * i + 2 * h], gates[8 * i + 2 * h + 1]);
+              }
+            }
+            gates_asked = false;
+            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+            __syncwarp(); // every lane has its row
+          }
+        }
+      };
+      if constexpr (kBoxes) {
+        take_gates();
+        if (!ok) {
+          break;
+        }
+        fetch_gates(1);
+      }
+      uint4 gate_raw[kBoxes ? 1 : 16]; // BF16 gates of this thread's 128 columns, fetched while the last PV is still running
+      if constexpr (!F32 && !kBoxes) {
         if (live) {
           const uint4 *gp = reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(p.gate) + out_base);
 #pragma unroll
@@ -1346,6 +1431,29 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
+      // (boxes) 64 columns of the warp's rows to the output; rows past the tile's last one lie outside the map or belong to no one
+      [[maybe_unused]] auto put_box = [&](const std::uint32_t (&packed)[kBoxes ? 32 : 1], int half) {
+        if constexpr (kBoxes) {
+          if (half == 1) {
+            if (lane == 0) {
+              tma_store_wait_read(); // the first half has left
+            }
+            __syncwarp();
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            *reinterpret_cast<uint4 *>(box_row + ((i ^ (lane & 7)) << 4)) =
+                make_uint4(packed[4 * i], packed[4 * i + 1], packed[4 * i + 2], packed[4 * i + 3]);
+          }
+          asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&w.output_map, static_cast<int>(head * kHeadDim + group * 128 + half * kBoxCols),
+                         static_cast<int>(row0 + (warp & 3) * 32), box);
+            tma_store_commit();
+          }
+        }
+      };
       ok = mbar_wait(bar(kBarPvDone + (g_last & 1U)), (g_last >> 1) & 1U, abort_flag);
       ok = __all_sync(0xFFFFFFFFU, ok);
       if (!ok) {
@@ -1459,10 +1567,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         inv = 1.0F / (l_sum + exchange[(sums + (group ^ 1)) * kTileRows + row]);
       }
       constexpr int kUnroll = F32 && Split ? 1 : 4; // BF16 gates sit in registers by piece
+      [[maybe_unused]] std::uint32_t packed_out[kBoxes ? 32 : 1]; // (boxes) 64 columns
 #pragma unroll kUnroll
       for (int c = 0; c < 4; ++c) {
         if (Split && (c < first_piece || c >= end_piece)) {
           continue;
+        }
+        if (kBoxes && c == 2) {
+          // the first 64 columns wait in registers until the gates of the others have left the box
+          take_gates();
+          if (!ok) {
+            break;
+          }
+          if (boxes) {
+            put_box(packed_out, 0);
+          }
         }
         std::uint32_t v[32];
         tmem_ld32(tmem_o + lane_base + group * 128 + c * 32, v);
@@ -1507,7 +1626,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           tcgen05_fence_before();
           arrive_on_leader(kBarOFree);
         }
-        if (live) {
+        if constexpr (kBoxes) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const float r0 = __uint_as_float(v[e]) * inv * gates[(c & 1) * 32 + e];
+            const float r1 = __uint_as_float(v[e + 1]) * inv * gates[(c & 1) * 32 + e + 1];
+            packed_out[(c & 1) * 16 + e / 2] = pack_bf16(r0, r1);
+          }
+          if (c == 3 && boxes) {
+            put_box(packed_out, 1);
+          }
+        } else if (live) {
           if constexpr (F32) {
 #pragma unroll
             for (int e = 0; e < 32; e += 8) {
@@ -1585,6 +1714,17 @@ __global__ void __launch_bounds__(kThreads, 1)
 #ifdef RIB200_TRACE
       traced_blocks += blocks;
 #endif
+    }
+    if constexpr (kBoxes) {
+      // nothing of this warp's is on its way any more when it leaves, also after a wait that ran out
+      if (gates_asked) {
+        const long long started = clock64();
+        while (!mbar_try_wait(gate_bar, gate_parity) && clock64() - started <= kWaitLimitCycles) {
+        }
+      }
+      if (lane == 0) {
+        tma_store_wait_all();
+      }
     }
   }
 
@@ -1758,6 +1898,13 @@ template <bool F32, bool Pair, int Parts, bool Window> void launch(const Prefill
     form.sinks = a.window.sinks;
     form.origin = origin;
     form.staged = staged ? 1U : 0U;
+    if (!F32) {
+      const cuuint64_t dims[2] = {static_cast<cuuint64_t>(a.query_heads) * kHeadDim, a.tokens};
+      const cuuint64_t strides[1] = {static_cast<cuuint64_t>(a.query_heads) * kHeadDim * 2};
+      const cuuint32_t box[2] = {kBoxCols, 32};
+      form.gate_map = make_map(const_cast<void *>(a.gate), 2, dims, strides, box);
+      form.output_map = make_map(a.output, 2, dims, strides, box);
+    }
     form.k_sink_map = k_map;
     form.v_sink_map = v_map;
     if (a.window.seen_sinks > 0) {

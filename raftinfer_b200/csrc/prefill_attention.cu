@@ -336,6 +336,11 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap *map, int c0, int
                "r"(c0), "r"(c1), "r"(c2), "r"(src)
                : "memory");
 }
+__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap *map, int c0, int c1) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];\n" ::"l"(reinterpret_cast<std::uint64_t>(map)),
+               "r"(c0), "r"(c1)
+               : "memory");
+}
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, int c0, int c1, std::uint32_t src) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];\n" ::"l"(
                    reinterpret_cast<std::uint64_t>(map)),
@@ -1215,7 +1220,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       };
-      fetch_gates(0);
+      if constexpr (kBoxes) {
+        if (boxes && lane == 0) { // the second half is asked into L2 by now: it has to come quickly when its turn is there
+          tma_prefetch_2d(&w.gate_map, static_cast<int>(head * kHeadDim + group * 128 + kBoxCols),
+                          static_cast<int>(row0 + (warp & 3) * 32));
+        }
+        if (blocks == 1) {
+          fetch_gates(0);
+        }
+      }
 
       float m_used = -INFINITY; // maximum the exponentials are taken against (scaled, base 2); same in both groups
       float l_sum = 0.0F;       // this thread's share of the row sum
@@ -1352,6 +1365,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_wait_st();
         tcgen05_fence_before();
         arrive_on_leader(kBarPFull + buf);
+        if (kBoxes && j == 0 && blocks > 1) {
+          fetch_gates(0); // by now the previous tile's outputs have left the box
+        }
         if (threadIdx.x == 0 && walk.iteration == 0) {
           RIB200_STAMP(j, 13); // P published
         }

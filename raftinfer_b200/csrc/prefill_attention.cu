@@ -80,6 +80,7 @@ constexpr int kThreads = 320;
 constexpr long long kWaitLimitCycles = 1LL << 30;
 constexpr float kScaleLog2e = 0.0625F * 1.4426950408889634F; // (1 / sqrt(256)) * log2(e)
 constexpr float kRescaleThreshold = 8.0F;
+constexpr float kNothingSeen = -1.0e30F; // maximum of a row that sees no key
 // Split form: an item shares its key blocks between two CTAs (or pairs) when it has at least this many.  The
 // hand-over of the partial tile costs about as much as five blocks, so where only part of a launch's items are long
 // (a rank's slice of the heads of a long prompt, tiles of 1 .. 32 blocks) the bar is higher.
@@ -1307,10 +1308,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         // the scale is positive: it commutes with the maximum.  A row that sees no key of this block (possible only
         // for the second half of a split item) gets a large negative finite maximum, so that its weights are zeros.
-        const float mx = fmaxf(fmaxf(mine, theirs) * kScaleLog2e, -1.0e30F);
+        const float mx = fmaxf(fmaxf(mine, theirs) * kScaleLog2e, kNothingSeen);
         // move the reference maximum only when it fell far behind; block 0 always sets it
         const bool move = mx > m_used + kRescaleThreshold;
-        if (__any_sync(0xFFFFFFFFU, move && j > 0)) {
+        // (A row that has seen no key so far has zeros in O.  Behind a window that is half of a tile's rows in its first block: 4096
+        // tokens, window 1024, 64.0 us when they were rescaled.)
+        if (__any_sync(0xFFFFFFFFU, move && j > 0 && (!Window || m_used > kNothingSeen))) {
           // rescale this warp's 32 rows of O (this group's 128 columns); PV(j-1) must have landed
           ok = mbar_wait(bar(kBarPvDone + ((g - 1) & 1U)), ((g - 1) >> 1) & 1U, abort_flag);
           ok = __all_sync(0xFFFFFFFFU, ok);
@@ -1417,16 +1420,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         fetch_gates(1);
       }
       uint4 gate_raw[kBoxes ? 1 : 16]; // BF16 gates of this thread's 128 columns, fetched while the last PV is still running
-      if constexpr (!F32 && !kBoxes) {
-        if (live) {
-          const uint4 *gp = reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(p.gate) + out_base);
+      // (windowed, split: the loads wait until the messages to the others are on their way, so that those are not behind them)
+      const bool gates_later = Window && Split && split_here;
+      auto load_gates = [&] {
+        if constexpr (!F32 && !kBoxes) {
+          if (live) {
+            const uint4 *gp = reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(p.gate) + out_base);
 #pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            if (i / 4 >= first_piece && i / 4 < end_piece) {
-              ld_global_v8(gp + i, gate_raw[i], gate_raw[i + 1]);
+            for (int i = 0; i < 16; i += 2) {
+              if (i / 4 >= first_piece && i / 4 < end_piece) {
+                ld_global_v8(gp + i, gate_raw[i], gate_raw[i + 1]);
+              }
             }
           }
         }
+      };
+      if (!gates_later) {
+        load_gates();
       }
       // FP32 gates cannot all wait in registers as the BF16 ones do: the first 32-column piece is fetched here, while
       // the last PV is still running, the other three are pulled into L2 and fetched one piece ahead further down
@@ -1543,6 +1553,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           tcgen05_fence_before();
           arrive_on_leader(kBarOFree);
           continue;
+        }
+        if (gates_later) {
+          load_gates();
         }
         const float *own_stat = reinterpret_cast<const float *>(smem); // any message's: they carry the same
         const float own_sum = own_stat[kTileRows + row] + own_stat[2 * kTileRows + row];

@@ -13,6 +13,7 @@ namespace rib200 {
 namespace {
 
 constexpr std::size_t kUnbounded = 0x7FFFFFFFU;
+constexpr std::uint32_t kWholeContext = 0xFFFFFFFFU;
 
 bool eight_bit_of(std::uint8_t cache_dtype, const char *unknown) {
   require(cache_dtype <= RIB200_KV_CACHE_E4M3, unknown);
@@ -28,7 +29,7 @@ std::size_t one_cache_bytes(std::size_t kv_heads, std::size_t rows, bool eight_b
 }
 
 std::uint32_t clamp_tokens(std::size_t tokens) { return static_cast<std::uint32_t>(std::min(tokens, kUnbounded)); }
-std::uint32_t window_of(std::size_t window_tokens) { return window_tokens == 0 ? kUnbounded : clamp_tokens(window_tokens); }
+std::uint32_t window_of(std::size_t window_tokens) { return window_tokens == 0 ? kWholeContext : clamp_tokens(window_tokens); }
 
 void aligned(const void *pointer, const char *message) {
   require(reinterpret_cast<std::uintptr_t>(pointer) % 16 == 0, message);

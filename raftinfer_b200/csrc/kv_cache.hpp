@@ -41,7 +41,7 @@ struct KvDecodeArgs {
   const std::uint32_t *positions;
   std::uint32_t batch;
   std::uint32_t query_heads;
-  std::uint32_t window; // 0x7FFFFFFF: the whole context
+  std::uint32_t window; // 0xFFFFFFFF: the whole context
   std::uint32_t sinks;
   bool activations_f32;
   void *workspace;

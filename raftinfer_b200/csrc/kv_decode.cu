@@ -17,7 +17,7 @@
 //
 // Arithmetic: mma.sync m16n8k16, tokens (for values: dims) as the 16 rows, and as the 8 columns four query heads in two parts
 // each, the value rounded to 16 bits and what is left of it, so that queries and weights count with 2^-16 of a value or
-// better.  (A matrix instruction with 64 rows and more would be filled by four heads to a sixteenth.)  BF16 rows
+// better (FP32 activations: 2^-22 and better).  (A matrix instruction with 64 rows and more would be filled by four heads to a sixteenth.)  BF16 rows
 // go into it as they are.  8-bit codes become FP16 in registers, which is exact; queries are scaled by a power of two to FP16's
 // range, the block's K scale multiplies the logits, and its V scale, relative to the largest one so far, the weights: every
 // scale is a power of two, so nothing is rounded by it.  Logits, maxima, sums and outputs are FP32.
@@ -392,10 +392,29 @@ __device__ __forceinline__ float4 gated(float4 v, float4 gate) {
                      v.w / (1.0F + expf(-gate.w)));
 }
 
+// Parts 0 and 1, 2 and 3 of two values in BF16: column parts `part` and `part` + 2.
+__device__ __forceinline__ void split4(float x, float y, int part, std::uint32_t &first, std::uint32_t &second) {
+  std::uint32_t parts[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 rounded = __floats2bfloat162_rn(x, y);
+    const float2 back = __bfloat1622float2(rounded);
+    parts[i] = *reinterpret_cast<const std::uint32_t *>(&rounded);
+    x -= back.x;
+    y -= back.y;
+  }
+  first = part != 0 ? parts[1] : parts[0];
+  second = part != 0 ? parts[3] : parts[2];
+}
+
 // A lane's 16 dims of a step's matrix operand, as the fragments want them.
 //   BF16: fragment ks, half: dims 16 ks + 8 half + 2 t, +1.   8 bit: fragment 4 s + w, half: dims 64 s + 16 t + 4 w + 2 half, +1.
+// FP32 queries over BF16 rows have four parts of eight bits: columns take parts 0 and 1, and in a second product into the same
+// sums parts 2 and 3 (two parts are off by 2^-17, ten times the error of FP32 sums).
 template <bool F32, bool EightBit> struct Query {
+  static constexpr bool kFourParts = F32 && !EightBit;
   std::uint32_t fragment[32];
+  std::uint32_t rest[kFourParts ? 32 : 1];
   float scale; // of head t: logit (base 2) = product * scale (* the block's K scale)
 
   // column g of the lane (g, t): head g / 2, part g & 1
@@ -417,7 +436,11 @@ template <bool F32, bool EightBit> struct Query {
             x = make_float2(__uint_as_float(raw << 16), __uint_as_float(raw & 0xFFFF0000U));
           }
         }
-        fragment[i] = split2<false>(x.x, x.y, part);
+        if constexpr (kFourParts) {
+          split4(x.x, x.y, part, fragment[i], rest[i]);
+        } else {
+          fragment[i] = split2<false>(x.x, x.y, part);
+        }
       }
       scale = 0.0625F * kLog2e;
     } else {
@@ -739,6 +762,9 @@ __global__ void __launch_bounds__(Shape<EightBit>::kWarps * 32, Shape<EightBit>:
           std::uint32_t a[4];
           ldmatrix_x4(address + ks * 32, a);
           mma<false>(s[ks & 3], a[0], a[1], a[2], a[3], q.fragment[2 * ks], q.fragment[2 * ks + 1]);
+          if constexpr (q.kFourParts) {
+            mma<false>(s[ks & 3], a[0], a[1], a[2], a[3], q.rest[2 * ks], q.rest[2 * ks + 1]);
+          }
         }
       }
       // both parts of head t's logits
@@ -848,8 +874,15 @@ __global__ void __launch_bounds__(Shape<EightBit>::kWarps * 32, Shape<EightBit>:
         const float w1 = __shfl_sync(0xFFFFFFFFU, weight_a, from + 4);
         const float w2 = __shfl_sync(0xFFFFFFFFU, weight_b, from);
         const float w3 = __shfl_sync(0xFFFFFFFFU, weight_b, from + 4);
-        const std::uint32_t b0 = split2<false>(w0, w1, part);
-        const std::uint32_t b1 = split2<false>(w2, w3, part);
+        std::uint32_t b0, b1;
+        [[maybe_unused]] std::uint32_t rest0, rest1;
+        if constexpr (q.kFourParts) {
+          split4(w0, w1, part, b0, rest0);
+          split4(w2, w3, part, b1, rest1);
+        } else {
+          b0 = split2<false>(w0, w1, part);
+          b1 = split2<false>(w2, w3, part);
+        }
         const std::uint32_t mi = lane >> 3;
         const std::uint32_t address = v_slot + (lane & 7U) * L::kPitch + (mi >> 1) * 512 + (mi & 1U) * 16;
 #pragma unroll
@@ -857,6 +890,9 @@ __global__ void __launch_bounds__(Shape<EightBit>::kWarps * 32, Shape<EightBit>:
           std::uint32_t a[4];
           ldmatrix_x4_trans(address + m * 32, a);
           mma<false>(oacc[m], a[0], a[1], a[2], a[3], b0, b1);
+          if constexpr (q.kFourParts) {
+            mma<false>(oacc[m], a[0], a[1], a[2], a[3], rest0, rest1);
+          }
         }
       }
     }

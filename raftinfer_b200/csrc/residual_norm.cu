@@ -3,10 +3,11 @@
 //   h = x + r,   y = h / sqrt(mean(h^2) + eps) * w,   codes = round(y / s),  s = 2^e of the group's largest |y|
 //
 // A CTA takes a row at a time, eight columns to a thread in each of one, two or four pieces; the row stays in registers
-// between the sum of squares and the output, all in FP32, one rounding per output.  Bytes: x, r read, h and the output
-// written, once each; bound by memory.  Many rows: all CTAs are resident, keep their columns' weights and fetch their next
-// row while the current one is reduced.  4096 rows of 4096 BF16 columns to 8 bits 21.9 us (5.4 TB/s), 2709 FP32 rows
-// to FP32 30.9 us (5.7 TB/s); a CTA for each row took 71.6 and 40.1.
+// between the sum of squares and the output.  h is FP32; codes are the value rounded once (see below), other outputs FP32
+// arithmetic rounded once.  Bytes: x, r read, h and the output written, once each; bound by memory.  Many rows: all CTAs are
+// resident, keep their columns' weights and fetch their next row while the current one is reduced.  4096 rows of 4096 columns:
+// BF16 to BF16 23.4 us (5.7 TB/s), BF16 to 8 bits 27.3 (4.3 TB/s, two thirds of the copy rate: issue slots, 21.9 before codes
+// were exact); 2709 FP32 rows to FP32 30.7 (5.8 TB/s).  A CTA for each row took 71.6 (8 bits) and 40.1 (FP32).
 
 #include "kv_cache.hpp"
 #include "residual_norm.hpp"
@@ -23,6 +24,7 @@ namespace rib200 {
 namespace {
 
 constexpr float kLargest = 3.4028234663852886e38F;
+constexpr std::uint32_t kNear = 4; // units of the last place
 
 // Eight neighbouring columns as they lie in memory, and as FP32.
 template <class T> struct alignas(16) Eight { std::uint32_t word[sizeof(T) * 2]; };
@@ -59,8 +61,9 @@ template <class T> __device__ __forceinline__ Eight<T> pack(const float (&v)[8])
   return out;
 }
 
-// maximum or sum over the CTA; `slots` holds a float for each warp, and no one may still read it
-template <class Op> __device__ __forceinline__ float over_block(float v, float *slots, Op op) {
+// Each warp's sum or maximum into `slots`, which holds a value for each of 16 warps (zeros for those that the CTA does not
+// have) and which no one may still read.
+template <class V, class Op> __device__ __forceinline__ void over_warps(V v, V *slots, Op op) {
 #pragma unroll
   for (int step = 16; step > 0; step /= 2) {
     v = op(v, __shfl_xor_sync(0xFFFFFFFFU, v, step));
@@ -69,17 +72,20 @@ template <class Op> __device__ __forceinline__ float over_block(float v, float *
     slots[threadIdx.x / 32] = v;
   }
   __syncthreads();
-  v = slots[0];
-  for (std::uint32_t w = 1; w < blockDim.x / 32; ++w) {
-    v = op(v, slots[w]);
-  }
-  return v;
 }
 
 // Group: columns that share a scale (32 or 128; 0 a whole row), -1 an output in T.
 template <class T, class W, int Pieces, int Group>
-__global__ void __launch_bounds__(512) residual_norm_kernel(const ResidualNormArgs p) {
-  __shared__ float slots[2][2][16]; // [row parity][sum, maximum][warp]
+__global__ void __launch_bounds__(sizeof(T) == 2 && Pieces <= 2 ? 256 : 512, sizeof(T) == 2 && Pieces <= 2 ? 4 : 1)
+    residual_norm_kernel(const ResidualNormArgs p) {
+  constexpr int kWarps = Pieces <= 2 ? 8 : 16;
+  __shared__ alignas(16) double sum_slots[2][16]; // [row parity][warp]
+  __shared__ alignas(16) float max_slots[2][16];
+  if (threadIdx.x < 32) {
+    sum_slots[threadIdx.x / 16][threadIdx.x % 16] = 0.0;
+    max_slots[threadIdx.x / 16][threadIdx.x % 16] = 0.0F;
+  }
+  __syncthreads();
   grid_dependency_wait();
   grid_dependents_may_launch();
   const std::uint32_t pieces = p.columns / 8;
@@ -109,11 +115,13 @@ __global__ void __launch_bounds__(512) residual_norm_kernel(const ResidualNormAr
       weight[i] = static_cast<const Eight<W> *>(p.weight)[piece];
     }
   }
-  const float columns = static_cast<float>(p.columns);
+  const double one_column = 1.0 / static_cast<double>(p.columns);
+  const double epsilon = static_cast<double>(p.epsilon);
   std::uint32_t parity = 0;
   for (std::size_t row = blockIdx.x; row < p.rows; row += gridDim.x, parity ^= 1U) {
     float h[Pieces][8];
-    float sum = 0.0F;
+    using Sum = std::conditional_t<(Group < 0), float, double>;
+    Sum sum = 0;
 #pragma unroll
     for (int i = 0; i < Pieces; ++i) {
       const std::uint32_t piece = threadIdx.x + i * blockDim.x;
@@ -129,7 +137,7 @@ __global__ void __launch_bounds__(512) residual_norm_kernel(const ResidualNormAr
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          sum = fmaf(h[i][e], h[i][e], sum);
+          sum = fma(static_cast<Sum>(h[i][e]), static_cast<Sum>(h[i][e]), sum);
         }
         if (p.residual_out != nullptr) {
           static_cast<Eight<T> *>(p.residual_out)[row * pieces + piece] = pack<T>(h[i]);
@@ -139,15 +147,54 @@ __global__ void __launch_bounds__(512) residual_norm_kernel(const ResidualNormAr
     if (row + gridDim.x < p.rows) {
       fetch(row + gridDim.x);
     }
-    sum = over_block(sum, slots[parity][0], [](float a, float b) { return a + b; });
-    const float factor = 1.0F / sqrtf(sum / columns + p.epsilon);
+    // The factor is common to a row, so its error moves all of the row's values towards a code's border together.  For codes the
+    // squares are summed in 64 bits (a few columns may hold most of the sum, so that errors do not average out).  The factor is an approximation f
+    // of m^(-1/2) and what Newton's step adds to it, f (1 - m f^2) / 2, and the products below carry their rounding along.
+    over_warps(static_cast<double>(sum), sum_slots[parity], [](double a, double b) { return a + b; });
+    double total = 0.0;
+#pragma unroll
+    for (int i = 0; i < kWarps; i += 2) {
+      const double2 two = reinterpret_cast<const double2 *>(sum_slots[parity])[i / 2];
+      total += two.x + two.y;
+    }
+    const double mean = fma(total, one_column, epsilon);
+    const float m = static_cast<float>(mean), m_rest = static_cast<float>(mean - static_cast<double>(m));
+    const float factor = rsqrtf(m);
+    const float square = factor * factor, square_rest = fmaf(factor, factor, -square);
+    const float factor_rest = 0.5F * factor * fmaf(-m, square_rest, fmaf(-m_rest, square, fmaf(-m, square, 1.0F)));
+    const float whole_factor = factor + factor_rest;
 #pragma unroll
     for (int i = 0; i < Pieces; ++i) {
       float w[8];
       unpack<W>(weight[i], w);
+      float y[8];
+      std::uint32_t near = 0xFFFFFFFFU;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        h[i][e] = h[i][e] * factor * w[e];
+        y[e] = h[i][e] * whole_factor * w[e];
+        near = min(near, (__float_as_uint(y[e]) + kNear) & 0x7FFFFU);
+      }
+      if constexpr (Group >= 0) {
+        // The middle between two codes, and the largest value of a scale, have nineteen zeros at the end, and y (three
+        // roundings) is within three units of its last place.  Where it comes near such a number (one value in 58000) it is worked out again with what the
+        // products left, and its last bit says on which side it lies: a code is the value rounded once.
+        if (near <= 2 * kNear) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float product = h[i][e] * w[e];
+            const float rest = fmaf(fmaf(h[i][e], w[e], -product), factor, product * factor_rest);
+            const float exact = fmaf(product, factor, rest);
+            const float left = fmaf(product, factor, -exact) + rest;
+            const std::uint32_t bits = __float_as_uint(exact);
+            const std::uint32_t beside = (left > 0.0F) == (exact > 0.0F) ? bits + 1 : bits - 1;
+            const bool middle = (bits & 0x7FFFFU) == 0 && exact != 0.0F && left != 0.0F;
+            y[e] = __uint_as_float(middle ? beside : bits);
+          }
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        h[i][e] = y[e];
       }
     }
     if constexpr (Group < 0) {
@@ -187,7 +234,12 @@ __global__ void __launch_bounds__(512) residual_norm_kernel(const ResidualNormAr
         for (int i = 1; i < Pieces; ++i) {
           row_amax = fmaxf(row_amax, amax[i]);
         }
-        row_amax = over_block(row_amax, slots[parity][1], [](float a, float b) { return fmaxf(a, b); });
+        over_warps(row_amax, max_slots[parity], [](float a, float b) { return fmaxf(a, b); });
+#pragma unroll
+        for (int i = 0; i < kWarps; i += 4) {
+          const float4 four = reinterpret_cast<const float4 *>(max_slots[parity])[i / 4];
+          row_amax = fmaxf(row_amax, fmaxf(fmaxf(four.x, four.y), fmaxf(four.z, four.w)));
+        }
 #pragma unroll
         for (int i = 0; i < Pieces; ++i) {
           amax[i] = row_amax;

@@ -54,7 +54,7 @@ class Batch:
                 self.after[i].store(length - 1, np.stack([self.k[i].numpy(), self.v[i].numpy()])[:, :, None])
         self.positions = [length - 1 if length else K.NO_POSITION for length in lengths]
         self.output = torch.full((n, heads, D), 7.0, device="cuda", dtype=self.query.dtype)
-        self.workspace = torch.empty(K.kv_decode_workspace_bytes(), device="cuda", dtype=torch.uint8)
+        self.workspace = torch.full((K.kv_decode_workspace_bytes(),), 0xFF, device="cuda", dtype=torch.uint8)  # not-a-numbers
         self.device_positions = torch.from_numpy(np.array(self.positions, dtype=np.uint32).view(np.int32)).cuda()
         if paged:
             self._place_pages(seed)
@@ -268,7 +268,7 @@ def test_a_cache_pointer_off_its_boundary_is_flagged_and_not_read():
 
 @KINDS
 def test_captured_steps_that_share_a_workspace(kind):
-    """Two steps of different batches in one graph each, one workspace, replayed in turn with positions that move."""
+    """Two steps of different batches in one graph each, one workspace, replayed in turn."""
     stream = torch.cuda.current_stream()
     batches = [Batch(kind, [700, 33], K.DTYPE_BF16, 61, paged=True), Batch(kind, [2000], K.DTYPE_BF16, 67)]
     shared = batches[0].workspace
@@ -286,6 +286,57 @@ def test_captured_steps_that_share_a_workspace(kind):
     assert K.device_status(stream) == 0
     for b in batches:
         b.check()
+
+
+@KINDS
+def test_a_captured_step_with_positions_that_move(kind):
+    """One graph, replayed with the token and its position rewritten in place: a context that grows from 250 to 262 tokens
+    (over a block and over a page) behind a window, beside an entry that turns into padding."""
+    stream, window, sinks = torch.cuda.current_stream(), 40, 3
+    b = Batch(kind, [250, 20], K.DTYPE_F32, 97, window=window, sinks=sinks, paged=True, poison=False)
+    pages = torch.arange(4, dtype=torch.int32)  # two pages a sequence
+    before = [Cache(kind, 4, 512), Cache(kind, 4, 512)]
+    for i, n in ((0, 249), (1, 19)):
+        before[i].store(0, normal(500 + i, 2, 4, n, D).numpy())
+    b.pool = to_device(np.concatenate([c.pages() for c in before]))
+    b.tables, b.pool_pages, b.max_blocks = pages.view(2, 2).cuda(), 4, 2
+    graph, first = torch.cuda.CUDAGraph(), True
+    for step in range(12):
+        for t, x in ((b.query, b.q), (b.key, b.k), (b.value, b.v), (b.gate, b.g)):
+            x.copy_(normal(1000 + 10 * step + x.shape[1], *x.shape))
+            t.copy_(x)
+        position = [249 + step, 19 + step if step < 5 else K.NO_POSITION]
+        b.device_positions.copy_(torch.from_numpy(np.array(position, dtype=np.uint32).view(np.int32)))
+        b.output.fill_(7.0)
+        if first:
+            b.run()  # what is captured has run once
+            torch.cuda.synchronize()
+            with torch.cuda.graph(graph, stream=stream):
+                b.run()
+            first = False
+        graph.replay()
+        torch.cuda.synchronize()
+        assert K.device_status(stream) == 0
+        for i in range(2):
+            if position[i] == K.NO_POSITION:
+                assert (b.output[i] == 7.0).all()
+                continue
+            before[i].store(position[i], np.stack([b.k[i].numpy(), b.v[i].numpy()])[:, :, None])
+            out, size, spread, total = attention(before[i], b.q[i:i + 1], b.g[i:i + 1], position[i], window, sinks)
+            assert ((b.output[i:i + 1].double() - out).abs() <= tolerance(out, size, spread, total, torch.float32)).all()
+        want = np.concatenate([c.pages() for c in before])
+        assert np.array_equal(from_device(b.pool, want), want)
+
+
+@KINDS
+def test_more_sequences_than_a_warp_has_lanes_for(kind):
+    lengths = [1 + (7 * i) % 40 for i in range(1500)]
+    lengths[3] = lengths[1111] = 0
+    b = Batch(kind, lengths, K.DTYPE_BF16, 101, kv_heads=1, group=1)
+    b.run()
+    torch.cuda.synchronize()
+    assert K.device_status(torch.cuda.current_stream()) == 0
+    b.check()
 
 
 @KINDS

@@ -184,6 +184,50 @@ def test_a_prompt_in_chunks_and_then_tokens(kind, paged):
 
 
 @KINDS
+@pytest.mark.parametrize("dtype", [K.DTYPE_BF16, K.DTYPE_F32], ids=["bf16", "f32"])
+def test_calls_one_behind_the_other_without_waiting(kind, dtype):
+    """Chunks and tokens enqueued on one stream with nothing between them, one workspace for all: outputs and the cache are
+    those of the same calls made one at a time."""
+    heads, window, sinks, capacity = 16, 150, 5, 600
+    stream = torch.cuda.current_stream()
+    chunks, total = [130, 17, 200, 1, 60], 408
+    new = [normal(i, total + 20, h, D).cuda().to(torch.float32 if dtype == K.DTYPE_F32 else torch.bfloat16)
+           for i, h in ((1, heads), (2, 4), (3, 4), (4, heads))]
+    scratch = torch.empty(1 << 22, device="cuda", dtype=torch.uint8)
+    capacities = torch.tensor([capacity], device="cuda", dtype=torch.int32)
+    positions = [torch.tensor([total + i], device="cuda", dtype=torch.int32) for i in range(20)]
+
+    def calls(wait):
+        cache = to_device(Cache(kind, 4, capacity).bytes)
+        pointer = torch.tensor([cache.data_ptr()], device="cuda")
+        output = torch.zeros_like(new[0])
+        torch.cuda.synchronize()
+        past = 0
+        for tokens in chunks:
+            rows = slice(past, past + tokens)
+            shape = K.Qwen35AttentionShape(tokens, heads, 4, D, capacity, past)
+            K.kv_attention_prefill(*[t[rows] for t in new], output[rows], cache, cache.numel() * cache.element_size(), scratch,
+                                   scratch.numel(), shape, window, sinks, dtype, kind, stream)
+            past += tokens
+            if wait:
+                torch.cuda.synchronize()
+        for i in range(20):
+            rows = slice(past + i, past + i + 1)
+            K.kv_batched_decode(*[t[rows] for t in new], output[rows], pointer, capacities, positions[i], 1, heads, 4, window,
+                                sinks, dtype, kind, scratch, scratch.numel(), stream)
+            if wait:
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        assert K.device_status(stream) == 0
+        return output, cache
+
+    (one, cache_one), (other, cache_other) = calls(True), calls(False)
+    assert torch.equal(cache_one, cache_other)
+    # (a prompt's sums do not depend on timing, a token's neither)
+    assert torch.equal(one, other) and torch.isfinite(one.float()).all()
+
+
+@KINDS
 def test_a_long_prompt_behind_a_window(kind):
     p = Prompt(kind, 6000, kv_heads=2, group=2, window=700, sinks=130)
     p.fill(0)

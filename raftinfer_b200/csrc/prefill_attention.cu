@@ -61,6 +61,7 @@ constexpr int kHeadDim = 256;
 constexpr int kTileRows = 128;  // query rows per CTA
 constexpr int kBlockKeys = 128; // keys per score tile
 constexpr int kHalfKeys = 64;   // keys per ring slot
+constexpr int kNarrowKeys = 32; // keys of a block of few sinks
 constexpr int kSlots = 5;
 constexpr int kBoxCols = 64;                              // 64 BF16 = one 128-byte swizzle row
 constexpr int kQBoxBytes = kTileRows * 128;               // 16 KiB
@@ -178,6 +179,9 @@ struct TileBlocks {
   std::uint32_t sinks;  // of the first kind, from block 0 on
   std::uint32_t window; // first block of the second kind
   std::uint32_t end;    // one behind the last
+  // The one block of the first kind has no visible key behind its first kNarrowKeys: its products are of that many keys (a few
+  // sinks in front of a window of 1024 are else a tenth of the tensor work).
+  bool narrow;
   __host__ __device__ std::uint32_t count() const { return sinks + end - window; }
   __host__ __device__ std::uint32_t block(std::uint32_t index) const {
     return index < sinks ? index : window + (index - sinks);
@@ -187,8 +191,9 @@ __host__ __device__ inline TileBlocks tile_blocks_of(std::uint32_t first, std::u
                                                      std::uint32_t sinks) {
   const std::uint32_t low_first = first + 1 > window ? first + 1 - window : 0U;
   const std::uint32_t low_last = last + 1 > window ? last + 1 - window : 0U;
-  return TileBlocks{((sinks < low_last ? sinks : low_last) + kBlockKeys - 1) / kBlockKeys, low_first / kBlockKeys,
-                    last / kBlockKeys + 1};
+  const std::uint32_t seen = sinks < low_last ? sinks : low_last;
+  return TileBlocks{(seen + kBlockKeys - 1) / kBlockKeys, low_first / kBlockKeys, last / kBlockKeys + 1,
+                    seen != 0 && seen <= kNarrowKeys};
 }
 
 __device__ __forceinline__ std::uint32_t smem_u32(const void *p) {
@@ -759,7 +764,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const std::uint32_t first = p.past + tile * kTileRows;
       return tile_blocks_of(first, first + tile_rows(tile) - 1, w.window, w.sinks);
     } else {
-      return TileBlocks{0, 0, tile_end(tile)};
+      return TileBlocks{0, 0, tile_end(tile), false};
     }
   };
   auto tile_blocks = [&](std::uint32_t tile) {
@@ -960,7 +965,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             } else {
               for (int b = 0; b < 4; ++b) {
                 tma_load_3d_pair(dst + b * kSlotBoxBytes, k_src, b * kBoxCols,
-                                 key0 + static_cast<int>(rank * kHalfKeys), static_cast<int>(kv_head), leader_bar);
+                                 key0 + static_cast<int>(rank * (is_sink && walked.narrow ? kNarrowKeys / 2 : kHalfKeys)),
+                                 static_cast<int>(kv_head), leader_bar);
               }
             }
             ++n;
@@ -1026,6 +1032,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr int kUnitRows = Pair ? 2 * kTileRows : kTileRows;
       constexpr std::uint32_t kIdescQk = instr_desc(kUnitRows, kBlockKeys, false);
       constexpr std::uint32_t kIdescPv = instr_desc(kUnitRows, kHeadDim, true);
+      constexpr std::uint32_t kIdescNarrow = instr_desc(kUnitRows, kNarrowKeys, false);
       // Descriptors are built once; inside the loops only a constant is added to the address field.
       const std::uint64_t q_desc = smem_desc(q_smem, 16, 1024);
       const std::uint64_t k_desc = smem_desc(ring, 16, 1024); // K-major, 8-row groups 1 KiB apart
@@ -1065,8 +1072,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         wait(kBarQFull, walk.iteration & 1U);
         // S[g & 1] = Q K_block^T.  Pair form: one slot, each CTA holding 64 of the block's 128 keys with all 256
         // dims in four 64-dim boxes.  Single form: two slots, each holding all 128 keys for half of the dims.
+        const bool narrow_first = Window && window_blocks(walk.tile()).narrow && first_block(walk.tile()) == 0;
         auto issue_qk = [&](std::uint32_t j) {
           const std::uint32_t g = g0 + j;
+          const std::uint32_t idesc = narrow_first && j == 0 ? kIdescNarrow : kIdescQk;
           if (walk.iteration == 0) {
             RIB200_STAMP(j, 0); // QK issue begins
           }
@@ -1079,7 +1088,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int ks = 0; ks < 16; ++ks) {
                 const std::uint32_t a_off = ((ks >> 2) * kQBoxBytes + (ks & 3) * 32) >> 4;
                 const std::uint32_t b_off = ((ks >> 2) * kSlotBoxBytes + (ks & 3) * 32) >> 4;
-                umma_ss_pair(d, q_desc + a_off, b0 + b_off, kIdescQk, ks > 0 ? 1U : 0U);
+                umma_ss_pair(d, q_desc + a_off, b0 + b_off, idesc, ks > 0 ? 1U : 0U);
               }
             }
             commit(kBarEmpty + slot);
@@ -1095,7 +1104,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int ks = 0; ks < 8; ++ks) {
                   const std::uint32_t a_off = ((ks >> 2) * kQBoxBytes + (ks & 3) * 32) >> 4;
                   const std::uint32_t b_off = ((ks >> 2) * kKeyBoxBytes + (ks & 3) * 32) >> 4;
-                  umma_ss(d, a0 + a_off, b0 + b_off, kIdescQk, (half > 0 || ks > 0) ? 1U : 0U);
+                  umma_ss(d, a0 + a_off, b0 + b_off, idesc, (half > 0 || ks > 0) ? 1U : 0U);
                 }
               }
               commit(kBarEmpty + slot);
@@ -1137,6 +1146,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (leader) {
 #pragma unroll
               for (int ks = 0; ks < 8; ++ks) {
+                if (ks >= kNarrowKeys / 16 && narrow_first && j == 0) {
+                  break;
+                }
                 const std::uint32_t a = tmem_s + (g & 1U) * kBlockKeys + ks * 8;
                 umma_ts_pair(tmem_o, a, b0 + ((ks * 2048) >> 4), kIdescPv, (j > 0 || ks > 0) ? 1U : 0U);
               }
@@ -1151,6 +1163,9 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (leader) {
 #pragma unroll
                 for (int ks = 0; ks < 4; ++ks) {
+                  if ((half > 0 || ks >= kNarrowKeys / 16) && narrow_first && j == 0) {
+                    break;
+                  }
                   const std::uint32_t a = tmem_s + (g & 1U) * kBlockKeys + half * 32 + ks * 8;
                   umma_ts(tmem_o, a, b0 + ((ks * 2048) >> 4), kIdescPv, (j > 0 || half > 0 || ks > 0) ? 1U : 0U);
                 }

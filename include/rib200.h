@@ -416,11 +416,13 @@ Rib200Status rib200_online_attention_decode_early_kv_fetch(const void *query, co
  *
  * Attention reads what the cache holds: the new tokens' rows are stored first, and 8-bit rows are used as rounded.  A query
  * at position p sees the tokens j <= p with j > p - window_tokens or j < sink_tokens; window_tokens == 0 is the whole
- * context.  What is not visible may hold anything in a single-token call; in a prompt call the rows that its first token
- * does not see (neither a sink nor in its window) may hold anything in an 8-bit or paged cache and have to be finite in a
- * contiguous BF16 one.  Pages with no visible row are not looked up.  Outputs are out = (attention) * sigmoid(gate).
+ * context.  Rows that no query of a call sees may hold anything, not-a-numbers too, and their pages are not looked up; the
+ * scale of the 8-bit block that a call's first row goes into has to be the one that the calls before left there, unless it is
+ * the block's first row.  Outputs are out = (attention) * sigmoid(gate).
  * Activations (query, key, value, gate, output) are BF16 or FP32; a prompt call rounds FP32 queries to BF16, and FP32
- * keys and values to the cache's type; a single-token call rounds keys and values alone. */
+ * keys and values to the cache's type; a single-token call rounds keys and values alone.  A prompt call rounds weights to
+ * BF16, and counts gates under -40 as -40.  A workspace serves one call at a time (calls on one stream may share one) and
+ * needs no preparation. */
 enum { RIB200_KV8_BLOCK_TOKENS = 16, RIB200_KV8_BLOCK_BYTES = 4112 };
 /* A batch entry of rib200_kv_batched_decode and rib200_kv_paged_decode with this position is skipped: nothing is stored and
  * its output row stays as it is. */
@@ -471,9 +473,10 @@ Rib200Status rib200_kv_paged_decode(const void *query, const void *key, const vo
  * qwen35_rms_norm behind the executor's residual addition (cpp/kernels/qwen35_primitives.cu:118-160) as one call, with an
  * output in 8 bits where the projection takes one: h = input + residual in FP32 (residual may be NULL),
  * residual_out = h in `dtype` (may be NULL; may be `residual` or `input` itself), y = h / sqrt(mean(h^2) + epsilon) * weight.
+ * `output` may be `input` itself where their types are the same; other overlaps are not allowed.
  * output_dtype == dtype: output = y, scales NULL, group_columns 0.  RIB200_DTYPE_E4M3: output holds codes [rows][columns]
  * and scales (FP32) [rows][columns / group_columns], the powers of two of the 8-bit cache for each group of 32 or 128
- * columns of a row; group_columns == 0 is one scale for the row.  dtype FP32, BF16 or FP16; weight FP32 or BF16;
+ * columns of a row; group_columns == 0 is one scale for the row.  A code is the value rounded once.  dtype FP32, BF16 or FP16; weight FP32 or BF16;
  * columns a multiple of 8 (of group_columns) up to 16384. */
 Rib200Status rib200_residual_rms_norm(const void *input, const void *residual, const void *weight, void *output,
                                       float *scales, void *residual_out, size_t rows, size_t columns,

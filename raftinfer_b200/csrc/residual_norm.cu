@@ -120,8 +120,7 @@ __global__ void __launch_bounds__(sizeof(T) == 2 && Pieces <= 2 ? 256 : 512, siz
   std::uint32_t parity = 0;
   for (std::size_t row = blockIdx.x; row < p.rows; row += gridDim.x, parity ^= 1U) {
     float h[Pieces][8];
-    using Sum = std::conditional_t<(Group < 0), float, double>;
-    Sum sum = 0;
+    double sum = 0.0;
 #pragma unroll
     for (int i = 0; i < Pieces; ++i) {
       const std::uint32_t piece = threadIdx.x + i * blockDim.x;
@@ -137,7 +136,7 @@ __global__ void __launch_bounds__(sizeof(T) == 2 && Pieces <= 2 ? 256 : 512, siz
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          sum = fma(static_cast<Sum>(h[i][e]), static_cast<Sum>(h[i][e]), sum);
+          sum = fma(static_cast<double>(h[i][e]), static_cast<double>(h[i][e]), sum);
         }
         if (p.residual_out != nullptr) {
           static_cast<Eight<T> *>(p.residual_out)[row * pieces + piece] = pack<T>(h[i]);
@@ -147,10 +146,10 @@ __global__ void __launch_bounds__(sizeof(T) == 2 && Pieces <= 2 ? 256 : 512, siz
     if (row + gridDim.x < p.rows) {
       fetch(row + gridDim.x);
     }
-    // The factor is common to a row, so its error moves all of the row's values towards a code's border together.  For codes the
-    // squares are summed in 64 bits (a few columns may hold most of the sum, so that errors do not average out).  The factor is an approximation f
-    // of m^(-1/2) and what Newton's step adds to it, f (1 - m f^2) / 2, and the products below carry their rounding along.
-    over_warps(static_cast<double>(sum), sum_slots[parity], [](double a, double b) { return a + b; });
+    // The squares are summed in 64 bits: large rows do not overflow, and the factor, whose error would move all of a row's
+    // values towards a code's border together, is good to 2^-45.  (A few columns may hold most of the sum, so that 32-bit errors
+    // do not average out.)  It is an approximation f of m^(-1/2) and what Newton's step adds to it, f (1 - m f^2) / 2.
+    over_warps(sum, sum_slots[parity], [](double a, double b) { return a + b; });
     double total = 0.0;
 #pragma unroll
     for (int i = 0; i < kWarps; i += 2) {
@@ -158,10 +157,17 @@ __global__ void __launch_bounds__(sizeof(T) == 2 && Pieces <= 2 ? 256 : 512, siz
       total += two.x + two.y;
     }
     const double mean = fma(total, one_column, epsilon);
-    const float m = static_cast<float>(mean), m_rest = static_cast<float>(mean - static_cast<double>(m));
-    const float factor = rsqrtf(m);
-    const float square = factor * factor, square_rest = fmaf(factor, factor, -square);
-    const float factor_rest = 0.5F * factor * fmaf(-m, square_rest, fmaf(-m_rest, square, fmaf(-m, square, 1.0F)));
+    float factor, factor_rest;
+    if (mean > 1.0e-30 && mean < 1.0e30) {
+      const float m = static_cast<float>(mean), m_rest = static_cast<float>(mean - static_cast<double>(m));
+      factor = rsqrtf(m);
+      const float square = factor * factor, square_rest = fmaf(factor, factor, -square);
+      factor_rest = 0.5F * factor * fmaf(-m, square_rest, fmaf(-m_rest, square, fmaf(-m, square, 1.0F)));
+    } else { // beyond what those products can hold; also zeros, infinities and not-a-numbers
+      const double wide = rsqrt(mean);
+      factor = static_cast<float>(wide);
+      factor_rest = isinf(mean) ? 0.0F : static_cast<float>(wide - static_cast<double>(factor));
+    }
     const float whole_factor = factor + factor_rest;
 #pragma unroll
     for (int i = 0; i < Pieces; ++i) {

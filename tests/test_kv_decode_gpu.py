@@ -329,6 +329,25 @@ def test_a_captured_step_with_positions_that_move(kind):
 
 
 @KINDS
+def test_pages_behind_four_gigabytes(kind):
+    """A pool of more than 2^32 bytes, the sequence's pages at its end and its beginning."""
+    page_bytes = K.kv_cache_bytes(4, PAGE, kind)
+    pool_pages = (1 << 32) // page_bytes + 9
+    b = Batch(kind, [600], K.DTYPE_F32, 103, paged=True)
+    pool = torch.zeros(pool_pages, *b.pool.shape[1:], device="cuda", dtype=b.pool.dtype)
+    where = torch.tensor([pool_pages - 1, 0, pool_pages - 3], device="cuda")
+    pool[where] = b.pool[b.tables[0].long()]
+    want = b.want_pool[b.tables[0].cpu().numpy()]
+    b.pool, b.pool_pages, b.tables = pool, pool_pages, where.int()[None]
+    b.run()
+    torch.cuda.synchronize()
+    assert K.device_status(torch.cuda.current_stream()) == 0
+    out, size, spread, total = attention(b.after[0], b.q, b.g, 599, 0, 0)
+    assert ((b.output.double() - out).abs() <= tolerance(out, size, spread, total, torch.float32)).all()
+    assert np.array_equal(from_device(pool[where], want), want)
+
+
+@KINDS
 def test_more_sequences_than_a_warp_has_lanes_for(kind):
     lengths = [1 + (7 * i) % 40 for i in range(1500)]
     lengths[3] = lengths[1111] = 0

@@ -125,6 +125,46 @@ def test_rows_of_zeros_and_of_extremes():
     check_codes(reference(x[1:], None, w)[1], 128, codes[1:], scales[1:])
 
 
+@pytest.mark.parametrize("dtype", [K.DTYPE_F32, K.DTYPE_BF16])
+def test_magnitudes_whose_squares_leave_32_bits(dtype):
+    """Rows around 1e25 and 1e-25 (with no epsilon), and one with an infinity: its finite columns become zeros."""
+    columns, stream = 520, torch.cuda.current_stream()
+    x = normal(3, 3, columns)
+    x[0] *= 1e25
+    x[1] *= 1e-25
+    x[2, 9] = float("inf")
+    x = x.to(TYPES[dtype]).cuda()
+    w = (1.0 + 0.2 * normal(4, columns)).cuda()
+    out, codes = torch.empty_like(x), torch.empty(3, columns, device="cuda", dtype=torch.uint8)
+    scales = torch.empty(3, 1, device="cuda")
+    K.residual_rms_norm(x, None, w, out, None, None, 3, columns, 0, 0.0, dtype, K.DTYPE_F32, dtype, stream)
+    K.residual_rms_norm(x, None, w, codes, scales, None, 3, columns, 0, 0.0, dtype, K.DTYPE_F32, K.DTYPE_E4M3, stream)
+    torch.cuda.synchronize()
+    h = x[:2].double()
+    y = h / torch.sqrt((h * h).mean(-1, keepdim=True)) * w.double()
+    check_plain(y, dtype, out[:2])
+    check_codes(y, 0, codes[:2], scales[:2])
+    assert torch.isnan(out[2]).nonzero().flatten().tolist() == [9]
+    assert (out[2, :9] == 0).all() and (out[2, 10:] == 0).all()
+
+
+def test_codes_are_the_value_rounded_once():
+    """Half a million values, outlier columns among them: every code is that of the 64-bit value, and so is every scale."""
+    rows, columns, stream = 256, 2048, torch.cuda.current_stream()
+    spread = torch.exp(0.5 * normal(5, columns)) * torch.where(normal(6, columns) > 3.0, 30.0, 1.0)
+    x, r = (normal(7, rows, columns) * spread).bfloat16().cuda(), (normal(8, rows, columns) * spread).bfloat16().cuda()
+    w = (1.0 + 0.2 * normal(9, columns)).cuda()
+    h = x.double() + r.double()
+    y = (h / torch.sqrt((h * h).mean(-1, keepdim=True) + EPSILON) * w.double()).cpu().numpy().reshape(rows, -1, 128)
+    codes, scales = torch.empty(rows, columns, device="cuda", dtype=torch.uint8), torch.empty(rows, columns // 128, device="cuda")
+    K.residual_rms_norm(x, r, w, codes, scales, None, rows, columns, 128, EPSILON, K.DTYPE_BF16, K.DTYPE_F32, K.DTYPE_E4M3,
+                        stream)
+    torch.cuda.synchronize()
+    want = np.vectorize(scale_for)(np.abs(y).max(-1))
+    assert np.array_equal(scales.cpu().numpy(), want)
+    assert np.array_equal(codes.cpu().numpy().reshape(y.shape), codes_for(y / want[..., None]))
+
+
 def test_a_not_a_number_stays_in_its_row():
     x, r, w = make(4, 256, K.DTYPE_F32)
     x[2, 5] = float("nan")

@@ -46,6 +46,7 @@ constexpr long long kWaitLimitCycles = 1LL << 28;
 constexpr float kLog2e = 1.4426950408889634F;
 constexpr float kLowest = -3.0e38F;
 constexpr float kWeightUnit = 32768.0F;
+constexpr std::uint32_t kNoSlot = 0xFFFFFFFFU;
 
 // Slots.  BF16: row pairs (1 KiB, one copy) at a pitch of 1040 bytes; the row index m of the matrix instruction stands for
 // token 2 (m % 8) + m / 8, so that the eight rows of an ldmatrix lie in eight different bank groups.  8 bit: groups of four
@@ -600,9 +601,8 @@ __global__ void __launch_bounds__(Shape<EightBit>::kWarps * 32, Shape<EightBit>:
   std::uint32_t step = plan.target != 0 ? start.index * plan.target : start.index;
   Count left = plan.target != 0 ? plan.target : plan.bound(blockIdx.x + 1) - plan.bound(blockIdx.x);
   bool first_row = true;
-  std::uint32_t used = 0;    // slots of this warp in the rows so far
-  std::uint32_t issued = 0;  // ... that have been asked for
-  std::uint32_t waited = 0;  // ... that have arrived
+  std::uint32_t issued = 0, issue_at = 0;                  // slots of this warp that have been asked for
+  std::uint32_t waited = 0, wait_at = 0, wait_parity = 0;  // ... that have arrived
   bool healthy = true;
 
   for (;;) {
@@ -616,23 +616,34 @@ __global__ void __launch_bounds__(Shape<EightBit>::kWarps * 32, Shape<EightBit>:
     const std::uint32_t my_slots = S::kHalves * my_steps;
     auto token_of = [&](std::uint32_t s) { return (s < row.sink_steps ? s : row.window_step + (s - row.sink_steps)) * kStep; };
 
+    // What this lane copies of a step, from the start of the cache or page on: a KiB of the K or V rows (8 bit: lanes 0 to 3 and 4
+    // to 7), two rows of the K plane (BF16).
+    const std::size_t plane_bytes = view.plane_bytes();
+    const std::size_t values_behind = view.kv_heads * plane_bytes; // V plane behind the K plane
+    const unsigned char *lane_base = view.base + head * plane_bytes +
+                                     (EightBit ? (lane & 3U) * 1024 + (lane & 4U ? values_behind : 0) : lane * 1024);
     // slot n of this row's part.  8 bit: K and V rows of the warp's step n; BF16: the K rows (n even) or V rows of step n / 2
     auto issue = [&](std::uint32_t n) {
       const std::uint32_t tok0 = token_of(begin + warp + n / S::kHalves * kWarps);
-      const std::uint32_t at = (used + n) % kSlots;
-      const std::uint32_t slot = ring + at * L::kBytes;
-      const std::uint32_t bar = bars + at * 8;
-      const unsigned char *plane = view.plane(n % S::kHalves, head, tok0);
-      const std::uint32_t r0 = view.row_in_plane(tok0);
+      const std::uint32_t slot = ring + issue_at * L::kBytes;
+      const std::uint32_t bar = bars + issue_at * 8;
+      issue_at = issue_at + 1 == kSlots ? 0 : issue_at + 1;
       ++issued;
+      const unsigned char *src = lane_base;
+      std::uint32_t row_in_plane = tok0;
       fence_proxy_async(); // earlier accesses to this slot are ordered before the copy
-      if (plane == nullptr) {
-        if (lane == 0) {
-          atomicOr(p.status, static_cast<unsigned int>(RIB200_DEVICE_PAGE_OUT_OF_RANGE));
-          mbarrier_expect_tx(bar, 0);
+      if (view.table != nullptr) {
+        const std::uint32_t page = __ldg(view.table + tok0 / kKvPageTokens);
+        row_in_plane = tok0 % kKvPageTokens;
+        src += page * (2 * values_behind);
+        if (page >= view.pool_pages) {
+          if (lane == 0) {
+            atomicOr(p.status, static_cast<unsigned int>(RIB200_DEVICE_PAGE_OUT_OF_RANGE));
+            mbarrier_expect_tx(bar, 0);
+          }
+          __syncwarp();
+          return;
         }
-        __syncwarp();
-        return;
       }
       if constexpr (EightBit) {
         if (lane == 0) {
@@ -640,10 +651,9 @@ __global__ void __launch_bounds__(Shape<EightBit>::kWarps * 32, Shape<EightBit>:
         }
         __syncwarp();
         if (lane < 8) {
-          const std::uint32_t piece = lane & 3U;
-          const unsigned char *src = plane + static_cast<std::size_t>(r0 / kStep) * kKv8BlockBytes + piece * 1024 +
-                                     (lane >= 4 ? view.kv_heads * view.plane_bytes() : 0);
-          bulk_copy_g2s(slot + (lane >= 4 ? L::kValues : 0U) + piece * L::kPitch, src, piece == 3 ? 1040 : 1024, bar, policy);
+          bulk_copy_g2s(slot + (lane & 4U ? L::kValues : 0U) + (lane & 3U) * L::kPitch,
+                        src + static_cast<std::size_t>(row_in_plane / kStep) * kKv8BlockBytes, (lane & 3U) == 3 ? 1040 : 1024,
+                        bar, policy);
         }
       } else {
         const std::uint32_t rows = min(kStep, row.pos + 1 - tok0);
@@ -652,18 +662,18 @@ __global__ void __launch_bounds__(Shape<EightBit>::kWarps * 32, Shape<EightBit>:
         }
         __syncwarp();
         if (2 * lane < rows) {
-          bulk_copy_g2s(slot + lane * L::kPitch, plane + static_cast<std::size_t>(r0 + 2 * lane) * 512,
+          bulk_copy_g2s(slot + lane * L::kPitch,
+                        src + static_cast<std::size_t>(row_in_plane) * 512 + (n & 1U ? values_behind : 0),
                         min(2U, rows - 2 * lane) * 512, bar, policy);
         }
       }
     };
-    auto wait = [&](std::uint32_t n) {
-      const std::uint32_t at = used + n;
-      const std::uint32_t bar = bars + at % kSlots * 8;
-      const std::uint32_t parity = (at / kSlots) & 1U;
-      if (!mbarrier_try_wait(bar, parity)) {
+    // The next slot, when its rows are here; kNoSlot if they do not come.
+    auto wait = [&] {
+      const std::uint32_t bar = bars + wait_at * 8;
+      if (!mbarrier_try_wait(bar, wait_parity)) {
         const long long started = clock64();
-        while (!mbarrier_try_wait(bar, parity)) {
+        while (!mbarrier_try_wait(bar, wait_parity)) {
           if (clock64() - started > kWaitLimitCycles) {
             healthy = false;
             break;
@@ -671,8 +681,16 @@ __global__ void __launch_bounds__(Shape<EightBit>::kWarps * 32, Shape<EightBit>:
         }
       }
       healthy = __all_sync(0xFFFFFFFFU, healthy);
-      waited += healthy ? 1U : 0U;
-      return healthy;
+      if (!healthy) {
+        return kNoSlot;
+      }
+      const std::uint32_t slot = ring + wait_at * L::kBytes;
+      ++waited;
+      if (++wait_at == kSlots) {
+        wait_at = 0;
+        wait_parity ^= 1U;
+      }
+      return slot;
     };
 
     const std::uint32_t early = min(my_slots, kSlots - 1);
@@ -723,10 +741,10 @@ __global__ void __launch_bounds__(Shape<EightBit>::kWarps * 32, Shape<EightBit>:
       if (S::kHalves * i + kSlots - 1 < my_slots) {
         issue(S::kHalves * i + kSlots - 1);
       }
-      if (!wait(S::kHalves * i)) {
+      const std::uint32_t k_slot = wait();
+      if (k_slot == kNoSlot) {
         break;
       }
-      const std::uint32_t k_slot = ring + (used + S::kHalves * i) % kSlots * L::kBytes;
       if (newest) {
         append(k_slot, 0, tok0);
       }
@@ -796,17 +814,18 @@ __global__ void __launch_bounds__(Shape<EightBit>::kWarps * 32, Shape<EightBit>:
       run_sum += weight_a + weight_b;
 
       // ---- V ----
+      std::uint32_t v_slot = k_slot + L::kValues;
       if constexpr (S::kHalves == 2) {
         fence_proxy_async();
         __syncwarp();
         if (2 * i + kSlots < my_slots) {
           issue(2 * i + kSlots);
         }
-        if (!wait(2 * i + 1)) {
+        v_slot = wait();
+        if (v_slot == kNoSlot) {
           break;
         }
       }
-      const std::uint32_t v_slot = S::kHalves == 2 ? ring + (used + 2 * i + 1) % kSlots * L::kBytes : k_slot + L::kValues;
       if (newest) {
         append(v_slot, 1, tok0);
       }
@@ -907,7 +926,6 @@ __global__ void __launch_bounds__(Shape<EightBit>::kWarps * 32, Shape<EightBit>:
         atomicOr(p.status, static_cast<unsigned int>(RIB200_DEVICE_WAIT_TIMED_OUT));
       }
     }
-    used += my_slots;
 
     run_sum += __shfl_xor_sync(0xFFFFFFFFU, run_sum, 4);
     run_sum += __shfl_xor_sync(0xFFFFFFFFU, run_sum, 8);

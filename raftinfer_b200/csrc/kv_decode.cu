@@ -8,16 +8,17 @@
 // Split.  The unit of work is a step, 16 tokens of one KV head.  The rows (sequence, KV head) of a batch are ragged and their
 // lengths are known on the device alone, so every CTA finds its share from the positions: with many rows the steps of all
 // rows, laid end to end, are cut into one equal piece per resident CTA, which may begin and end inside a row; with few rows
-// (at most an eighth of the CTAs) each row is cut into pieces of its own, so that no CTA has two.  (24 sequences of 2 K to 8 K
-// tokens, 96 rows: 75 us cut by rows, 50 end to end; 9 sequences, 36 rows: end to end costs a second prologue.)  What a CTA
+// (at most an eighth of the CTAs) each row is cut into pieces of its own, so that no CTA has two.  (8-bit sequences of 2 K to
+// 8 K tokens, four rows each, us by rows and end to end: 2 sequences 13.8 and 20.6, 9 26.0 and 28.0, 12 34.4 and 32.6, 24 66.6
+// and 48.8, 36 117 and 66.4; the rule's 36 rows of 296 CTAs lie between 9 and 12.)  What a CTA
 // knows of a row that others share goes to the workspace as (maximum, sum, normalised values); a second kernel puts the
 // parts of a row together.  A row that one CTA has to itself is written directly.
 //
 // Inside a CTA the warps take the steps of its piece in turn, each with a private ring of shared-memory slots filled by bulk
 // copies two or three slots ahead; they meet once at the end of a row.
 //
-// Measured in replayed graphs: 8 bit, 131000 tokens 50.6 us (5.3 TB/s), 64 sequences of 1 K to 32 K 339 us (6.5 TB/s, the copy
-// rate; 386 in long runs at the power cap), BF16 behind a window of 4096 168 us (6.2 TB/s), 777 tokens 8.4 us.
+// Measured in replayed graphs: 8 bit, 131000 tokens 50.6 us (5.3 TB/s), 64 sequences of 1 K to 32 K 343 us (6.5 TB/s, the copy
+// rate; 380 over two seconds, when the power cap has brought the SM clock to 1.68 GHz, where BF16 rows take 685), BF16 behind a window of 4096 168 us (6.2 TB/s), 777 tokens 8.4 us.
 //
 // Arithmetic: mma.sync m16n8k16, tokens (for values: dims) as the 16 rows, and as the 8 columns four query heads in two parts
 // each, the value rounded to 16 bits and what is left of it, so that queries and weights count with 2^-16 of a value or

@@ -62,7 +62,7 @@ enum {
   RIB200_DEVICE_POSITION_OUT_OF_RANGE = 1u << 1,    /* *device_position >= max_context_tokens */
   RIB200_DEVICE_WAIT_TIMED_OUT = 1u << 2,           /* a bounded on-device wait gave up */
   RIB200_DEVICE_PAGE_OUT_OF_RANGE = 1u << 3,        /* a block table names a page the pool does not hold */
-  RIB200_DEVICE_POINTER_MISALIGNED = 1u << 4,       /* a pointer read on the device is off its required boundary */
+  RIB200_DEVICE_POINTER_MISALIGNED = 1u << 4,       /* a pointer read on the device is off its boundary, or null */
   RIB200_DEVICE_DECAY_OUT_OF_RANGE = 1u << 5        /* gated delta, 64 tokens or more: decays grow too much, see there */
 };
 
@@ -454,8 +454,9 @@ Rib200Status rib200_kv_paged_prefill(const void *query, const void *key, const v
 /* One token for each sequence of a batch, as rib200_batched_decode_attention: query, gate, output
  * [batch][query_heads][256], key, value [batch][kv_heads][256]; 1 to 4 query heads per KV head.  kv_caches,
  * max_context_tokens and positions are device arrays of `batch` entries; a position outside its cache (other than
- * RIB200_NO_POSITION) sets RIB200_DEVICE_POSITION_OUT_OF_RANGE and the entry is skipped.  Two entries may share rows that
- * both only read, not the row (8-bit: the block) that either writes. */
+ * RIB200_NO_POSITION) sets RIB200_DEVICE_POSITION_OUT_OF_RANGE and the entry is skipped; a cache pointer that is null or
+ * off a 16-byte boundary sets RIB200_DEVICE_POINTER_MISALIGNED and its entry is skipped (beside RIB200_NO_POSITION it may be
+ * anything).  Two entries may share rows that both only read, not the row (8-bit: the block) that either writes. */
 Rib200Status rib200_kv_batched_decode(const void *query, const void *key, const void *value, const void *gate,
                                       void *output, void *const *kv_caches, const uint32_t *max_context_tokens,
                                       const uint32_t *positions, size_t batch, size_t query_heads, size_t kv_heads,
@@ -476,8 +477,8 @@ Rib200Status rib200_kv_paged_decode(const void *query, const void *key, const vo
  * `output` may be `input` itself where their types are the same; other overlaps are not allowed.
  * output_dtype == dtype: output = y, scales NULL, group_columns 0.  RIB200_DTYPE_E4M3: output holds codes [rows][columns]
  * and scales (FP32) [rows][columns / group_columns], the powers of two of the 8-bit cache for each group of 32 or 128
- * columns of a row; group_columns == 0 is one scale for the row.  A code is the value rounded once.  dtype FP32, BF16 or FP16; weight FP32 or BF16;
- * columns a multiple of 8 (of group_columns) up to 16384. */
+ * columns of a row; group_columns == 0 is one scale for the row.  A code is the value rounded once.
+ * dtype FP32, BF16 or FP16; weight FP32 or BF16; columns a multiple of 8 (of group_columns) up to 16384. */
 Rib200Status rib200_residual_rms_norm(const void *input, const void *residual, const void *weight, void *output,
                                       float *scales, void *residual_out, size_t rows, size_t columns,
                                       size_t group_columns, float epsilon, int32_t dtype, int32_t weight_dtype,

@@ -146,7 +146,7 @@ __device__ __forceinline__ std::uint32_t kv_refusal(const KvCaches &c, const KvV
   const std::uint32_t capacity = c.tables != nullptr ? c.max_blocks * kKvPageTokens : view.rows;
   std::uint32_t why = 0;
   // the pointers lie in device memory: the host cannot see them
-  why = reinterpret_cast<std::uintptr_t>(view.base) % 16 != 0 ? RIB200_DEVICE_POINTER_MISALIGNED : why;
+  why = view.base == nullptr || reinterpret_cast<std::uintptr_t>(view.base) % 16 != 0 ? RIB200_DEVICE_POINTER_MISALIGNED : why;
   why = pos >= capacity ? RIB200_DEVICE_POSITION_OUT_OF_RANGE : why;
   return pos == RIB200_NO_POSITION ? kKvPadding : why;
 }

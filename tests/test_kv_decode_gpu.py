@@ -267,6 +267,25 @@ def test_a_cache_pointer_off_its_boundary_is_flagged_and_not_read():
 
 
 @KINDS
+def test_a_null_cache_pointer_is_flagged_and_not_read(kind):
+    b = Batch(kind, [40, 300, 0], K.DTYPE_BF16, 59)
+    b.pointers[0] = 0
+    b.pointers[2] = 0  # beside padding a pointer may be anything
+    b.after[0] = b.before[0]
+    b.run()
+    torch.cuda.synchronize()
+    assert K.device_status(torch.cuda.current_stream()) == K.DEVICE_POINTER_MISALIGNED
+    assert (b.output[0] == 7.0).all()
+    b.lengths[0] = 0
+    b.check()
+    b.pointers[0] = b.caches[0].data_ptr()
+    b.device_positions[0] = -1  # padding
+    b.run()
+    torch.cuda.synchronize()
+    assert K.device_status(torch.cuda.current_stream()) == 0
+
+
+@KINDS
 def test_captured_steps_that_share_a_workspace(kind):
     """Two steps of different batches in one graph each, one workspace, replayed in turn."""
     stream = torch.cuda.current_stream()

@@ -18,14 +18,15 @@
 // copies two or three slots ahead; they meet once at the end of a row.
 //
 // Measured in replayed graphs: 8 bit, 131000 tokens 50.6 us (5.3 TB/s), 64 sequences of 1 K to 32 K 343 us (6.5 TB/s, the copy
-// rate; 380 over two seconds, when the power cap has brought the SM clock to 1.68 GHz, where BF16 rows take 685), BF16 behind a window of 4096 168 us (6.2 TB/s), 777 tokens 8.4 us.
+// rate; 380 over two seconds, when the power cap has brought the SM clock to 1.68 GHz, where BF16 rows take 685),
+// BF16 behind a window of 4096 168 us (6.2 TB/s), 777 tokens 8.4 us.
 //
 // Arithmetic: mma.sync m16n8k16, tokens (for values: dims) as the 16 rows, and as the 8 columns four query heads in two parts
 // each, the value rounded to 16 bits and what is left of it, so that queries and weights count with 2^-16 of a value or
 // better (FP32 activations: 2^-22 and better).  (A matrix instruction with 64 rows and more would be filled by four heads
-// to a sixteenth.)  BF16 rows go into it as they are.  8-bit codes become FP16 in registers, which is exact; queries are scaled by a power of two to FP16's
-// range, the block's K scale multiplies the logits, and its V scale, relative to the largest one so far, the weights: every
-// scale is a power of two, so nothing is rounded by it.  Logits, maxima, sums and outputs are FP32.
+// to a sixteenth.)  BF16 rows go into it as they are.  8-bit codes become FP16 in registers, which is exact; queries are
+// scaled by a power of two to FP16's range, the block's K scale multiplies the logits, and its V scale, relative to the
+// largest one so far, the weights: every scale is a power of two, so nothing is rounded by it.  Logits, maxima, sums and outputs are FP32.
 //
 // The new token's row belongs to the last step of its row: the warp that has that step rounds the row, writes it to the cache
 // and into its slot, and rounds the block's older rows again if the block's scale grew.

@@ -182,8 +182,9 @@ __global__ void __launch_bounds__(sizeof(T) == 2 && Pieces <= 2 ? 256 : 512, siz
       }
       if constexpr (Group >= 0) {
         // The middle between two codes, and the largest value of a scale, have nineteen zeros at the end, and y (three
-        // roundings) is within three units of its last place.  Where it comes near such a number (one value in 58000) it is worked out again with what the
-        // products left, and its last bit says on which side it lies: a code is the value rounded once.
+        // roundings) is within three units of its last place.  Where it comes near such a number (one value in 58000) it is
+        // worked out again with what the products left, and its last bit says on which side it lies: a code is the value
+        // rounded once.
         if (near <= 2 * kNear) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) {

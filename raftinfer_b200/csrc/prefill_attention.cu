@@ -90,6 +90,11 @@ constexpr std::uint32_t kSplitMinBlocksLate = 20;
 // ... and between four from here on, where half of the GPU stays free: 17 tokens behind 2688 (FP32, with the steps in
 // front) 33.6 us with two shares and 26.9 with four, 100 behind 4000 37.1 and 29.3; two tiles, 201 behind 1500, 28.8 and 29.0.
 constexpr std::uint32_t kQuarterMinBlocks = 8;
+// Windowed form, four shares that fill the GPU (two tiles of 16 heads).  Clusters of eight, pairs in quarters, have 15 places and
+// would need 16, and a second round costs more than it gives (201 tokens behind 1500 24.2 us in halves, 36.6 so); single CTAs in
+// clusters of four fit.  256 tokens, us in halves and in four: 9 blocks 20.0 and 21.2, 11 21.1 and 21.2, 12 22.5 and 21.5, 33
+// 35.5 and 30.9, 129 93.4 and 68.1; FP32, 11 blocks, 25.3 and 23.6.
+constexpr std::uint32_t kQuarterMinBlocksAll = 11;
 
 // barrier indices (8 bytes each) inside the barrier block
 enum : int {
@@ -2084,6 +2089,16 @@ void launch_prefill_attention(const PrefillArgs &args, cudaStream_t stream) {
                                                                 : configure_once<kF32, false, 4, kWindow>());
       return tiles * args.query_heads / (pair ? 2 : 1) <= fit;
     };
+    const bool single_quarters = kWindow && split && !quarters &&
+                                 4 * tiles * args.query_heads <= static_cast<std::uint32_t>(sm_count) &&
+                                 first_tile_blocks >= kQuarterMinBlocksAll;
+    if constexpr (kWindow) {
+      if (single_quarters &&
+          tiles * args.query_heads <= static_cast<std::uint32_t>(configure_once<kF32, false, 4, kWindow>())) {
+        launch<kF32, false, 4, kWindow>(args, stream);
+        return;
+      }
+    }
     if (quarters && quarters_fit()) {
       if (pair) {
         launch<kF32, true, 4, kWindow>(args, stream);

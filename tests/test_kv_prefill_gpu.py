@@ -140,6 +140,20 @@ def test_fp32_activations(kind, tokens, past, window, sinks):
 
 
 @KINDS
+@pytest.mark.parametrize("dtype", [K.DTYPE_BF16, K.DTYPE_F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("paged", [False, True], ids=["contiguous", "paged"])
+@pytest.mark.parametrize("tokens,past,window,sinks,kv_heads,group", [
+    (129, 1152, 0, 0, 4, 4), (130, 1270, 0, 0, 4, 4), (256, 1281, 0, 0, 4, 4), (255, 4001, 0, 0, 4, 4), (200, 3000, 1280, 4, 4, 4),
+    (131, 3000, 1290, 140, 4, 4), (100, 1500, 0, 0, 8, 4), (128, 2000, 1400, 33, 16, 2), (90, 1500, 0, 0, 4, 9), (201, 1500, 0, 0, 3, 5),
+    (200, 1700, 1500, 7, 1, 16)])
+def test_two_tiles_and_many_keys(kind, paged, dtype, tokens, past, window, sinks, kv_heads, group):
+    """Chunks whose items are cut into two or four shares, or whose heads are too many for four."""
+    p = Prompt(kind, past + tokens, kv_heads=kv_heads, group=group, window=window, sinks=sinks, paged=paged, dtype=dtype)
+    p.fill(past)
+    p.chunk(tokens)
+
+
+@KINDS
 @pytest.mark.parametrize("kv_heads,group", [(1, 1), (2, 3), (1, 8), (3, 2), (8, 2)])
 def test_head_layouts(kind, kv_heads, group):
     for tokens, past, window, sinks in ((200, 0, 0, 0), (150, 900, 140, 6)):

@@ -6,8 +6,8 @@
 // between the sum of squares and the output.  h is FP32; codes are the value rounded once (see below), other outputs FP32
 // arithmetic rounded once.  Bytes: x, r read, h and the output written, once each; bound by memory.  Many rows: all CTAs are
 // resident, keep their columns' weights and fetch their next row while the current one is reduced.  4096 rows of 4096 columns:
-// BF16 to BF16 23.4 us (5.7 TB/s), BF16 to 8 bits 27.3 (4.3 TB/s, two thirds of the copy rate: issue slots, 21.9 before codes
-// were exact); 2709 FP32 rows to FP32 30.7 (5.8 TB/s).  A CTA for each row took 71.6 (8 bits) and 40.1 (FP32).
+// BF16 to BF16 23.4 us (5.7 TB/s), BF16 to 8 bits 27.0 (4.4 TB/s, two thirds of the copy rate: issue slots are 67 % busy, and warps
+// wait for the row's barrier and the group's shuffles; 21.9 before codes were exact); 2709 FP32 rows to FP32 30.7 (5.8 TB/s).  A CTA for each row took 71.6 (8 bits) and 40.1 (FP32).
 
 #include "kv_cache.hpp"
 #include "residual_norm.hpp"

@@ -150,8 +150,8 @@ struct PrefillWindow {
   std::uint32_t sinks;
   std::uint32_t low;        // first token of the first query's window
   std::uint32_t seen_sinks; // sinks in front of the last query's window
-  // null, or BF16 [K, V][kv head][staged_rows][256] with tokens [0, seen_sinks) and [low, past + tokens): attention reads this
-  // copy and the chunk's rows in it, and writes no cache
+  // null, or BF16 [K, V][kv head][staged_rows][256] with tokens [0, seen_sinks) from row 0 and [low, past + tokens) from row
+  // min(seen_sinks, low) on: attention reads this copy and the chunk's rows in it, and writes no cache
   void *staged;
   std::uint32_t staged_rows;
 };

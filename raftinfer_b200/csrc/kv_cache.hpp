@@ -74,8 +74,12 @@ inline KvVisible kv_visible(std::uint32_t tokens, std::uint32_t past, std::uint3
   const std::uint32_t low_last = context > window ? context - window : 0U;
   return KvVisible{sinks < low_last ? sinks : low_last, past + 1 > window ? past + 1 - window : 0U};
 }
-// Staged BF16 rows of a chunk, [K, V][kv head][row]: its sinks, then tokens [low, past + tokens).
-inline std::size_t kv_staged_rows(const KvVisible &seen, std::size_t context) { return seen.sinks + (context - seen.low); }
+// Staged BF16 rows of a chunk, [K, V][kv head][row]: its sinks, then tokens [low, past + tokens).  Sinks that reach into the first
+// query's window are there once: what is visible is then one run of tokens, and token t is row t.
+inline std::uint32_t kv_staged_low(const KvVisible &seen) { return seen.sinks < seen.low ? seen.sinks : seen.low; } // row of `low`
+inline std::size_t kv_staged_rows(const KvVisible &seen, std::size_t context) {
+  return kv_staged_low(seen) + (context - seen.low);
+}
 
 #ifdef __CUDACC__
 // The block scale for a largest finite magnitude of `amax`: 2^e with e in [-100, 119] least such that amax <= 448 * 2^e;

@@ -25,9 +25,10 @@ struct KvStoreArgs {
   std::uint32_t tokens, past;
   std::uint32_t sink_blocks;  // blocks of 16 tokens [0, sink_blocks), then [window_block, ...)
   std::uint32_t window_block;
-  std::uint32_t seen_sinks, seen_low;
-  void *staged; // BF16 [K, V][kv head][staged_rows][256]: tokens [0, seen_sinks), then from seen_low on
+  std::uint32_t seen_low;
+  void *staged; // BF16 [K, V][kv head][staged_rows][256]: tokens [0, seen_sinks), from row staged_low on those from seen_low on
   std::uint32_t staged_rows;
+  std::uint32_t staged_low;
   unsigned int *status;
 };
 
@@ -185,11 +186,11 @@ template <bool F32, bool EightBit> __global__ void __launch_bounds__(kThreads) k
 #pragma unroll
   for (int j = 0; j < kPieces; ++j) {
     const uint4 raw = pack8(x[j]);
-    if (token < p.seen_sinks) {
+    if (token < p.staged_low) { // (sinks behind it lie in the window: the rows below)
       *reinterpret_cast<uint4 *>(stage + static_cast<std::size_t>(token) * kKvHeadDim + dim0 + 64 * j) = raw;
     }
     if (token >= p.seen_low) {
-      *reinterpret_cast<uint4 *>(stage + static_cast<std::size_t>(token - p.seen_low + p.seen_sinks) * kKvHeadDim + dim0 +
+      *reinterpret_cast<uint4 *>(stage + static_cast<std::size_t>(token - p.seen_low + p.staged_low) * kKvHeadDim + dim0 +
                                  64 * j) = raw;
     }
   }
@@ -203,10 +204,10 @@ void launch_kv_store(const KvPrefillArgs &a, cudaStream_t stream) {
   p.tokens = a.tokens;
   p.past = a.past;
   const KvVisible seen = kv_visible(a.tokens, a.past, a.window, a.sinks);
-  p.seen_sinks = seen.sinks;
   p.seen_low = seen.low;
   p.staged = a.workspace;
   p.staged_rows = static_cast<std::uint32_t>(kv_staged_rows(seen, a.past + a.tokens));
+  p.staged_low = kv_staged_low(seen);
   // every block with a visible row once: those of the sinks, then those from the first window on
   p.sink_blocks = (seen.sinks + kKv8BlockTokens - 1) / kKv8BlockTokens;
   p.window_block = seen.low / kKv8BlockTokens > p.sink_blocks ? seen.low / kKv8BlockTokens : p.sink_blocks;

@@ -1933,7 +1933,7 @@ template <bool F32, bool Pair, int Parts, bool Window> void launch(const Prefill
   const std::uint32_t origin = Window ? a.window.low : 0U;
   const std::uint32_t plane_rows = staged ? a.window.staged_rows : a.max_context_tokens;
   auto *rows = staged ? static_cast<__nv_bfloat16 *>(a.window.staged) : cache;
-  auto *window_rows = rows + static_cast<std::size_t>(staged ? a.window.seen_sinks : origin) * kHeadDim;
+  auto *window_rows = rows + static_cast<std::size_t>(staged ? std::min(a.window.seen_sinks, origin) : origin) * kHeadDim;
   const std::size_t plane = static_cast<std::size_t>(a.kv_heads) * plane_rows * kHeadDim;
   const cuuint64_t kv_dims[3] = {kHeadDim, context - origin, a.kv_heads};
   const cuuint64_t kv_strides[2] = {kHeadDim * 2, static_cast<cuuint64_t>(plane_rows) * kHeadDim * 2};

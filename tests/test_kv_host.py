@@ -28,7 +28,8 @@ def test_sizes():
     workspace = lambda window, sinks, kind=K.KV_E4M3, paged=False: K.kv_prefill_workspace_bytes(shape, window, sinks, kind, paged)
     assert workspace(0, 0) == rows(3100) and workspace(0, 9) == rows(3100)
     assert workspace(1000, 0) == rows(1099) and workspace(1000, 5) == rows(1104) and workspace(1, 0) == rows(100)
-    assert workspace(1000, 2200) == rows(1099 + 2100)  # sinks that the last query's window has passed
+    # sinks up to 2099 (the last query's window has passed them) and tokens from 2001 on: 2100 + 1099 - 99 that are both
+    assert workspace(1000, 2200) == rows(3100)
     assert workspace(1000, 5, K.KV_BF16) == 0 and workspace(1000, 5, K.KV_BF16, True) == rows(1104)
     assert K.kv_decode_workspace_bytes() > 0
     for call, code in ((lambda: K.kv_cache_bytes(0, 1, K.KV_BF16), K.INVALID_ARGUMENT),
@@ -240,3 +241,17 @@ def test_the_model_of_the_scale():
         assert scale_for(np.nextafter(448.0 * 2.0 ** e, np.inf)) == 2.0 ** (e + 1)
         assert scale_for(225.0 * 2.0 ** e) == 2.0 ** e and scale_for(224.0 * 2.0 ** e) == 2.0 ** (e - 1)
     assert scale_for(0.0) == 2.0 ** -100 == scale_for(2.0 ** -140) and scale_for(2.0 ** 127.9) == 2.0 ** 119
+
+
+@pytest.mark.parametrize("cache_dtype", [K.KV_BF16, K.KV_E4M3])
+def test_a_prompt_workspace_holds_each_visible_row_once(cache_dtype):
+    """Sinks that lie in the first token's window, next to it, and in front of it: never more rows than the call sees."""
+    row = 2 * 4 * 256 * 2
+    for tokens, past, window, sinks in ((988, 0, 83, 163), (988, 0, 83, 905), (988, 0, 83, 2000), (100, 500, 200, 301),
+                                        (100, 500, 200, 300), (100, 500, 200, 302), (100, 500, 200, 0), (100, 500, 200, 350),
+                                        (100, 500, 0, 0), (100, 500, 1000, 7), (1, 500, 1, 500), (1, 0, 1, 1)):
+        first_low = max(0, past + 1 - window) if window else 0
+        last_low = max(0, past + tokens - window) if window else 0
+        seen = set(range(first_low, past + tokens)) | set(range(min(sinks, last_low)))
+        shape = K.Qwen35AttentionShape(tokens, 16, 4, 256, 4096, past)
+        assert K.kv_prefill_workspace_bytes(shape, window, sinks, cache_dtype, True) == len(seen) * row, (tokens, past, window, sinks)

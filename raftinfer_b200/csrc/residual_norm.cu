@@ -4,10 +4,11 @@
 //
 // A CTA takes a row at a time, eight columns to a thread in each of one, two or four pieces; the row stays in registers
 // between the sum of squares and the output.  h is FP32; codes are the value rounded once (see below), other outputs FP32
-// arithmetic rounded once.  Bytes: x, r read, h and the output written, once each; bound by memory.  Many rows: all CTAs are
-// resident, keep their columns' weights and fetch their next row while the current one is reduced.  4096 rows of 4096 columns:
-// BF16 to BF16 23.4 us (5.7 TB/s), BF16 to 8 bits 27.0 (4.4 TB/s, two thirds of the copy rate: issue slots are 67 % busy, and warps
-// wait for the row's barrier and the group's shuffles; 21.9 before codes were exact); 2709 FP32 rows to FP32 30.7 (5.8 TB/s).  A CTA for each row took 71.6 (8 bits) and 40.1 (FP32).
+// arithmetic rounded once, for rows of any magnitude.  Bytes: x, r read, h and the output written, once each; bound by memory.
+// Many rows: all CTAs are resident, keep their columns' weights and fetch their next row while the current one is reduced.
+// 4096 rows of 4096 columns: BF16 to BF16 23.3 us (5.8 TB/s), BF16 to 8 bits 27 (4.4 TB/s, two thirds of the copy rate: issue
+// slots, and warps that wait for the row's barrier and the group's shuffles; 21.9 with codes that one value in a million misses);
+// 2709 FP32 rows to FP32 30.5 (5.8 TB/s).  A CTA for each row took 71.6 (8 bits) and 40.1 (FP32).
 
 #include "kv_cache.hpp"
 #include "residual_norm.hpp"
@@ -74,6 +75,32 @@ template <class V, class Op> __device__ __forceinline__ void over_warps(V v, V *
   __syncthreads();
 }
 
+// Mean of a row's squares, from the warps' sums, plus epsilon.
+template <int Warps>
+__device__ __forceinline__ double mean_of(const double *slots, double one_column, double epsilon) {
+  double total = 0.0;
+#pragma unroll
+  for (int i = 0; i < Warps; i += 2) {
+    const double2 two = reinterpret_cast<const double2 *>(slots)[i / 2];
+    total += two.x + two.y;
+  }
+  return fma(total, one_column, epsilon);
+}
+// m^(-1/2), good to the last place but one: m = r 4^k with r in [1/2, 2), an approximation, and Newton's step twice.
+__device__ __forceinline__ double wide_factor(double m) {
+  if (!(m > 0.0) || m > 1.0e300) { // zeros, infinities, not-a-numbers; the squares of FP32 numbers are in between
+    return static_cast<double>(rsqrtf(static_cast<float>(m)));
+  }
+  const int k = (__double2hiint(m) >> 21) - 511;
+  const double r = __hiloint2double(__double2hiint(m) - (k << 21), __double2loint(m));
+  double f = static_cast<double>(rsqrtf(static_cast<float>(r)));
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    f = fma(0.5 * f, fma(-r * f, f, 1.0), f);
+  }
+  return __hiloint2double(__double2hiint(f) - (k << 20), __double2loint(f));
+}
+
 // Group: columns that share a scale (32 or 128; 0 a whole row), -1 an output in T.
 template <class T, class W, int Pieces, int Group>
 __global__ void __launch_bounds__(sizeof(T) == 2 && Pieces <= 2 ? 256 : 512, sizeof(T) == 2 && Pieces <= 2 ? 4 : 1)
@@ -117,6 +144,18 @@ __global__ void __launch_bounds__(sizeof(T) == 2 && Pieces <= 2 ? 256 : 512, siz
   }
   const double one_column = 1.0 / static_cast<double>(p.columns);
   const double epsilon = static_cast<double>(p.epsilon);
+  // |w| <= 2^16 keeps h * factor * w apart from what underflows: where h * factor (|h| factor <= 2^7) is under the smallest normal
+  // number, y is under 2^-110 and its code 0 at the smallest scale.
+  bool large_weights = false;
+#pragma unroll
+  for (int i = 0; i < (Group >= 0 ? Pieces : 0); ++i) {
+    float w[8];
+    unpack<W>(weight[i], w);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      large_weights = large_weights || !(fabsf(w[e]) <= 65536.0F);
+    }
+  }
   std::uint32_t parity = 0;
   for (std::size_t row = blockIdx.x; row < p.rows; row += gridDim.x, parity ^= 1U) {
     float h[Pieces][8];
@@ -147,28 +186,28 @@ __global__ void __launch_bounds__(sizeof(T) == 2 && Pieces <= 2 ? 256 : 512, siz
       fetch(row + gridDim.x);
     }
     // The squares are summed in 64 bits: large rows do not overflow, and the factor, whose error would move all of a row's
-    // values towards a code's border together, is good to 2^-45.  (A few columns may hold most of the sum, so that 32-bit errors
-    // do not average out.)  It is an approximation f of m^(-1/2) and what Newton's step adds to it, f (1 - m f^2) / 2.
+    // values towards a code's border together, is good to the last place.  (A few columns may hold most of the sum, so that 32-bit
+    // errors do not average out.)  It is an approximation f of m^(-1/2) and what Newton's step adds to it, f (1 - m f^2) / 2.
     over_warps(sum, sum_slots[parity], [](double a, double b) { return a + b; });
-    double total = 0.0;
-#pragma unroll
-    for (int i = 0; i < kWarps; i += 2) {
-      const double2 two = reinterpret_cast<const double2 *>(sum_slots[parity])[i / 2];
-      total += two.x + two.y;
+    const double mean = mean_of<kWarps>(sum_slots[parity], one_column, epsilon);
+    // y = h scale w factor.  8 bit: scale is 1, and factor is a not-a-number where these products may leave FP32's range.  Else
+    // scale is a power of two that brings the row to about one (2^126 and 2^-126 at most), so that they do not.
+    float scale = 1.0F;
+    float factor = __uint_as_float(0x7FFFFFFFU);
+    double scaled = mean;
+    if (Group < 0 && mean > 0.0 && mean < 1.0e300) {
+      const int k = min(max((__double2hiint(mean) >> 21) - 511, -126), 126);
+      scale = __uint_as_float(static_cast<std::uint32_t>(127 - k) << 23);
+      scaled = __hiloint2double(__double2hiint(mean) - (k << 21), __double2loint(mean));
     }
-    const double mean = fma(total, one_column, epsilon);
-    float factor, factor_rest;
-    if (mean > 1.0e-30 && mean < 1.0e30) {
-      const float m = static_cast<float>(mean), m_rest = static_cast<float>(mean - static_cast<double>(m));
+    if (Group < 0 || (!large_weights && mean > 1.0e-30 && mean < 1.0e30)) {
+      const float m = static_cast<float>(scaled), m_rest = static_cast<float>(scaled - static_cast<double>(m));
       factor = rsqrtf(m);
-      const float square = factor * factor, square_rest = fmaf(factor, factor, -square);
-      factor_rest = 0.5F * factor * fmaf(-m, square_rest, fmaf(-m_rest, square, fmaf(-m, square, 1.0F)));
-    } else { // beyond what those products can hold; also zeros, infinities and not-a-numbers
-      const double wide = rsqrt(mean);
-      factor = static_cast<float>(wide);
-      factor_rest = isinf(mean) ? 0.0F : static_cast<float>(wide - static_cast<double>(factor));
+      if (Group >= 0 || (m > 0.0F && m < kLargest)) {
+        const float square = factor * factor, square_rest = fmaf(factor, factor, -square);
+        factor = fmaf(0.5F * factor, fmaf(-m, square_rest, fmaf(-m_rest, square, fmaf(-m, square, 1.0F))), factor);
+      }
     }
-    const float whole_factor = factor + factor_rest;
 #pragma unroll
     for (int i = 0; i < Pieces; ++i) {
       float w[8];
@@ -177,25 +216,34 @@ __global__ void __launch_bounds__(sizeof(T) == 2 && Pieces <= 2 ? 256 : 512, siz
       std::uint32_t near = 0xFFFFFFFFU;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        y[e] = h[i][e] * whole_factor * w[e];
+        y[e] = Group < 0 ? h[i][e] * scale * w[e] * factor : h[i][e] * factor * w[e];
         near = min(near, (__float_as_uint(y[e]) + kNear) & 0x7FFFFU);
       }
       if constexpr (Group >= 0) {
         // The middle between two codes, and the largest value of a scale, have nineteen zeros at the end, and y (three
-        // roundings) is within three units of its last place.  Where it comes near such a number (one value in 58000) it is
-        // worked out again with what the products left, and its last bit says on which side it lies: a code is the value
-        // rounded once.
+        // roundings) is within three units of its last place.  Where it comes near such a number (one value in 58000; zeros are
+        // what they are) its piece is worked out again in 64 bits, and the last bit says on which side of it the value lies: a
+        // code is the value rounded once.  So is every value of a row whose factor, or of a thread whose weights, may take the
+        // products out of FP32's range: factor and y are then the not-a-number whose bits but the sign are ones, which looks the
+        // same.
+        bool again = false;
         if (near <= 2 * kNear) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const float product = h[i][e] * w[e];
-            const float rest = fmaf(fmaf(h[i][e], w[e], -product), factor, product * factor_rest);
-            const float exact = fmaf(product, factor, rest);
-            const float left = fmaf(product, factor, -exact) + rest;
-            const std::uint32_t bits = __float_as_uint(exact);
-            const std::uint32_t beside = (left > 0.0F) == (exact > 0.0F) ? bits + 1 : bits - 1;
-            const bool middle = (bits & 0x7FFFFU) == 0 && exact != 0.0F && left != 0.0F;
-            y[e] = __uint_as_float(middle ? beside : bits);
+            again = again || (y[e] != 0.0F && ((__float_as_uint(y[e]) + kNear) & 0x7FFFFU) <= 2 * kNear);
+          }
+        }
+        if (again) {
+          const double wide = wide_factor(mean_of<kWarps>(sum_slots[parity], one_column, epsilon));
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const double exact = static_cast<double>(h[i][e]) * static_cast<double>(w[e]) * wide;
+            y[e] = static_cast<float>(exact);
+            // within 2^-50 of such a number, about what the sum of squares leaves uncertain, a value counts as the number
+            const double left = exact - static_cast<double>(y[e]);
+            const std::uint32_t bits = __float_as_uint(y[e]);
+            const bool middle = (bits & 0x7FFFFU) == 0 && fabsf(y[e]) <= kLargest && fabs(left) > 0x1p-50 * fabs(exact);
+            y[e] = middle ? __uint_as_float((left > 0.0) == (exact > 0.0) ? bits + 1 : bits - 1) : y[e];
           }
         }
       }

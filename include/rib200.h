@@ -421,8 +421,9 @@ Rib200Status rib200_online_attention_decode_early_kv_fetch(const void *query, co
  * the block's first row.  Outputs are out = (attention) * sigmoid(gate).
  * Activations (query, key, value, gate, output) are BF16 or FP32; a prompt call rounds FP32 queries to BF16, and FP32
  * keys and values to the cache's type; a single-token call rounds keys and values alone.  A prompt call rounds weights to
- * BF16, and counts gates under -40 as -40.  A workspace serves one call at a time (calls on one stream may share one) and
- * needs no preparation. */
+ * BF16, and counts gates under -40 as -40; a single-token call over an 8-bit cache keeps 2^-22 of a weight, or 2^-40 of the
+ * head's largest product of a weight and its block's V scale if that is more, in place of the weight times its scale.
+ * A workspace serves one call at a time (calls on one stream may share one) and needs no preparation. */
 enum { RIB200_KV8_BLOCK_TOKENS = 16, RIB200_KV8_BLOCK_BYTES = 4112 };
 /* A batch entry of rib200_kv_batched_decode and rib200_kv_paged_decode with this position is skipped: nothing is stored and
  * its output row stays as it is. */

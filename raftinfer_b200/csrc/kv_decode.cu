@@ -25,8 +25,11 @@
 // each, the value rounded to 16 bits and what is left of it, so that queries and weights count with 2^-16 of a value or
 // better (FP32 activations: 2^-22 and better).  (A matrix instruction with 64 rows and more would be filled by four heads
 // to a sixteenth.)  BF16 rows go into it as they are.  8-bit codes become FP16 in registers, which is exact; queries are
-// scaled by a power of two to FP16's range, the block's K scale multiplies the logits, and its V scale, relative to the
-// largest one so far, the weights: every scale is a power of two, so nothing is rounded by it.  Logits, maxima, sums and outputs are FP32.
+// scaled by a power of two to FP16's range, the block's K scale multiplies the logits, and its V scale the weights.  What is
+// held of a weight is relative to the largest product of a weight and its block's V scale so far: two parts have 22 bits down
+// to 2^-18 of that, and what is 2^-40 of it vanishes, however the blocks' scales compare.  Maxima are rounded up to
+// integers and scales are powers of two, so nothing is rounded by moving from one to the other.  Logits, maxima, sums and
+// outputs are FP32.
 //
 // The new token's row belongs to the last step of its row: the warp that has that step rounds the row, writes it to the cache
 // and into its slot, and rounds the block's older rows again if the block's scale grew.
@@ -731,9 +734,11 @@ __global__ void __launch_bounds__(Shape<EightBit>::kWarps * 32, Shape<EightBit>:
     for (int i = 0; i < 16; ++i) {
       oacc[i][0] = oacc[i][1] = oacc[i][2] = oacc[i][3] = 0.0F;
     }
-    float run_max = kLowest;                 // of head t, base 2
+    float run_max = kLowest;                 // of head t, base 2; 8 bit: rounded up to an integer
     float run_sum = 0.0F;                    // this lane's share of head t's sum
-    float v_scale = EightBit ? __uint_as_float(27U << 23) : 1.0F; // 2^-100: the largest V scale so far
+    // 8 bit, of head t: 2^unit is the unit of the sums of values.  The largest weight (relative to 2^run_max) times the V scale
+    // of its block so far, rounded up to a power of two; from -100 to 119 once there is one.
+    [[maybe_unused]] float unit = kLowest;
 
     for (std::uint32_t i = 0; i < my_steps; ++i) {
       const std::uint32_t tok0 = token_of(begin + warp + i * kWarps);
@@ -802,18 +807,25 @@ __global__ void __launch_bounds__(Shape<EightBit>::kWarps * 32, Shape<EightBit>:
       step_max = fmaxf(step_max, __shfl_xor_sync(0xFFFFFFFFU, step_max, 4));
       step_max = fmaxf(step_max, __shfl_xor_sync(0xFFFFFFFFU, step_max, 8));
       step_max = fmaxf(step_max, __shfl_xor_sync(0xFFFFFFFFU, step_max, 16));
+      if constexpr (EightBit) {
+        step_max = ceilf(step_max);
+      }
       if (__any_sync(0xFFFFFFFFU, step_max > run_max)) {
         const float new_max = fmaxf(run_max, step_max);
         const float rescale = fast_exp2(run_max - new_max);
         run_sum *= rescale;
-        run_max = new_max;
+        if constexpr (EightBit) {
+          unit -= new_max - run_max;
+        } else {
 #pragma unroll
-        for (int m = 0; m < 16; ++m) {
+          for (int m = 0; m < 16; ++m) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            oacc[m][e] *= rescale;
+            for (int e = 0; e < 4; ++e) {
+              oacc[m][e] *= rescale;
+            }
           }
         }
+        run_max = new_max;
       }
       float weight_a = fast_exp2(logit_a - run_max);
       float weight_b = fast_exp2(logit_b - run_max);
@@ -850,10 +862,13 @@ __global__ void __launch_bounds__(Shape<EightBit>::kWarps * 32, Shape<EightBit>:
       // The weights as the other operand: lane (g, t) gives column g (head g / 2, part g & 1) for four tokens.
       const int part = g & 1;
       if constexpr (EightBit) {
-        const float scale = lds_float(v_slot + kSlotScale);
-        if (scale > v_scale) {
-          const float rescale = v_scale * kv8_inverse(scale);
-          v_scale = scale;
+        const float v_exponent =
+            static_cast<float>(static_cast<int>(__float_as_uint(lds_float(v_slot + kSlotScale)) >> 23) - 127);
+        const float step_unit = v_exponent + (step_max - run_max);
+        if (__any_sync(0xFFFFFFFFU, step_unit > unit)) {
+          const float new_unit = fmaxf(unit, step_unit);
+          const float rescale = fast_exp2(unit - new_unit);
+          unit = new_unit;
 #pragma unroll
           for (int m = 0; m < 16; ++m) {
 #pragma unroll
@@ -862,11 +877,9 @@ __global__ void __launch_bounds__(Shape<EightBit>::kWarps * 32, Shape<EightBit>:
             }
           }
         }
-        // weights times the block's scale relative to the largest, times 2^15: FP16 then holds what is 2^-40 of the largest
-        // and keeps 22 bits in two parts down to 2^-29
-        const float relative = scale * kv8_inverse(v_scale) * kWeightUnit;
-        weight_a *= relative;
-        weight_b *= relative;
+        // the weights times the block's scale in that unit: 2^15 at most
+        weight_a = fast_exp2((logit_a - run_max) + (v_exponent - unit)) * kWeightUnit;
+        weight_b = fast_exp2((logit_b - run_max) + (v_exponent - unit)) * kWeightUnit;
         // tokens 4 t .. 4 t + 3: token b3 b2 b1 b0 is row b1 ? b : a of the lane with g = b2 b0 b3
         const int from = (((t & 1) << 2) | (t >> 1)) * 4 + (g >> 1);
         const float w0 = __shfl_sync(0xFFFFFFFFU, weight_a, from);
@@ -958,15 +971,16 @@ __global__ void __launch_bounds__(Shape<EightBit>::kWarps * 32, Shape<EightBit>:
       warp_max[warp * kGroup + t] = run_max;
       warp_sum[warp * kGroup + t] = run_sum;
     }
-    const float normalise = run_sum == 0.0F ? 0.0F : (EightBit ? v_scale * (1.0F / kWeightUnit) / run_sum : 1.0F / run_sum);
+    const float normalise = run_sum == 0.0F ? 0.0F : (EightBit ? (1.0F / kWeightUnit) / run_sum : 1.0F / run_sum);
     {
       float *dst = warp_out + (warp * kGroup + t) * kMergePitch;
       if constexpr (EightBit) {
+        const float scale = fast_exp2(unit);
+        auto value = [&](int m, int e) { return (oacc[m][e] + oacc[m][e + 1]) * normalise * scale; };
 #pragma unroll
         for (int m = 0; m < 16; m += 2) {
           *reinterpret_cast<float4 *>(dst + 128 * (m >> 3) + 16 * g + 2 * (m & 7)) =
-              make_float4((oacc[m][0] + oacc[m][1]) * normalise, (oacc[m][2] + oacc[m][3]) * normalise,
-                          (oacc[m + 1][0] + oacc[m + 1][1]) * normalise, (oacc[m + 1][2] + oacc[m + 1][3]) * normalise);
+              make_float4(value(m, 0), value(m, 2), value(m + 1, 0), value(m + 1, 2));
         }
       } else {
 #pragma unroll

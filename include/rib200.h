@@ -423,6 +423,10 @@ Rib200Status rib200_online_attention_decode_early_kv_fetch(const void *query, co
  * keys and values to the cache's type; a single-token call rounds keys and values alone.  A prompt call rounds weights to
  * BF16, and counts gates under -40 as -40; a single-token call over an 8-bit cache keeps 2^-22 of a weight, or 2^-40 of the
  * head's largest product of a weight and its block's V scale if that is more, in place of the weight times its scale.
+ * Rows that are seen should be finite.  In a BF16 cache an infinity or a not-a-number counts as itself in a single-token call:
+ * a logit of minus infinity is a weight of zero, an infinite value an infinite output in its dim.  A prompt call takes
+ * 128 queries and 128 keys at a time and weights of zero for what is hidden: such a value may make its dim a not-a-number in
+ * all queries around it, those in front of it too.  (What no query of the call sees is not touched by either.)
  * A workspace serves one call at a time (calls on one stream may share one) and needs no preparation. */
 enum { RIB200_KV8_BLOCK_TOKENS = 16, RIB200_KV8_BLOCK_BYTES = 4112 };
 /* A batch entry of rib200_kv_batched_decode and rib200_kv_paged_decode with this position is skipped: nothing is stored and

@@ -1,4 +1,6 @@
-"""Single-token attention over rows of very different magnitudes, against a plain 64-bit model."""
+"""Single-token attention over rows of very different magnitudes and over rows with infinities, against a plain 64-bit model."""
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -178,5 +180,61 @@ def test_magnitudes_at_the_ends_of_the_scales():
         values[:, 64:] *= 2.0 ** -90
 
     b = Rows(K.KV_E4M3, [100, 800] + MANY, K.DTYPE_F32, 250, edit)
+    b.run()
+    b.check_range()
+
+
+LENGTHS = [33, 700, 1, 3001, 18]
+
+
+@DTYPES
+@pytest.mark.parametrize("paged", [False, True], ids=["contiguous", "paged"])
+@pytest.mark.parametrize("kv_heads,group", [(2, 4), (2, 3), (1, 1)])
+def test_keys_that_are_infinite(dtype, paged, kv_heads, group):
+    """A logit of minus infinity is a weight of zero; one of plus infinity makes its heads not-a-numbers."""
+    def edit(i, keys, values):
+        n = keys.shape[1]
+        if n > 1:
+            keys[:, n // 2, 0] = -math.inf
+            keys[:, 0, 0] = -math.inf
+        if n == 700:
+            keys[:, n - 1, 0] = -math.inf
+        if n == 18:
+            keys[0, 3, 0] = math.inf
+
+    b = Rows(K.KV_BF16, LENGTHS, dtype, 260, edit, kv_heads=kv_heads, group=group, paged=paged)
+    b.run()
+    b.check_range()
+    assert torch.isfinite(b.output[:4].float()).all() and torch.isnan(b.output[4, 0].float()).all()
+
+
+@DTYPES
+@pytest.mark.parametrize("paged", [False, True], ids=["contiguous", "paged"])
+@pytest.mark.parametrize("lengths", [LENGTHS, [40 + 13 * i for i in range(30)]], ids=["few", "many"])
+def test_values_that_are_infinite(dtype, paged, lengths):
+    """An infinity in a dim makes that dim's output infinite, two of unlike sign or a not-a-number a not-a-number, no other."""
+    def edit(i, keys, values):
+        n = keys.shape[1]
+        values[:, n // 2, 5] = math.inf
+        values[:, n - 1, 9] = -math.inf
+        values[:, 0, 200], values[:, n // 3, 200] = math.inf, -math.inf
+        values[0, n // 4, 255] = math.nan
+        if n > 1:
+            keys[:, n // 4, 0] = -math.inf
+
+    b = Rows(K.KV_BF16, lengths, dtype, 270, edit, kv_heads=2, paged=paged)
+    b.run()
+    b.check_range()
+
+
+@DTYPES
+def test_infinities_that_the_window_hides(dtype):
+    def edit(i, keys, values):
+        n = keys.shape[1]
+        for hidden in range(5, n - 50):
+            keys[:, hidden, 0], values[:, hidden, 3] = math.inf, -math.inf
+        values[:, n - 10, 4] = math.inf
+
+    b = Rows(K.KV_BF16, [700, 77, 300], dtype, 280, edit, kv_heads=1, window=50, sinks=5)
     b.run()
     b.check_range()

@@ -442,7 +442,8 @@ Rib200Status rib200_kv_prefill_workspace_bytes(const Rib200AttentionShape *shape
 Rib200Status rib200_kv_decode_workspace_bytes(size_t *bytes);
 
 /* A chunk of shape->tokens >= 1 tokens behind shape->past_tokens on one sequence's cache: query, gate, output
- * [tokens][query_heads][256], key, value [tokens][kv_heads][256], query_heads a multiple of kv_heads. */
+ * [tokens][query_heads][256], key, value [tokens][kv_heads][256], query_heads a multiple of kv_heads.  At most 65535 * 128
+ * tokens in a call and 2^23 in its context. */
 Rib200Status rib200_kv_attention_prefill(const void *query, const void *key, const void *value, const void *gate,
                                          void *output, void *kv_cache, size_t kv_cache_bytes, void *workspace,
                                          size_t workspace_bytes, const Rib200AttentionShape *shape,

@@ -1,6 +1,6 @@
 // Host side of the rib200_kv_* calls and of rib200_residual_rms_norm: sizes, argument checks and dispatch.
-// What they narrow: head_dim 256; a prompt's context up to 2^23 tokens, 256 KV heads and 1024 query heads; up to four query
-// heads for a KV head in single-token calls; tensor pointers 16-byte aligned.
+// What they narrow: head_dim 256; a prompt's context up to 2^23 tokens, a chunk of it up to 65535 * 128, 256 KV heads and 1024
+// query heads; up to four query heads for a KV head in single-token calls; tensor pointers 16-byte aligned.
 
 #include "kv_cache.hpp"
 #include "residual_norm.hpp"
@@ -62,6 +62,7 @@ void check_prefill_shape(const Rib200AttentionShape *shape) {
   unsupported(s.head_dim == kKvHeadDim, "KV attention: built for head_dim 256");
   unsupported(s.query_heads <= 1024 && s.kv_heads <= 256, "KV attention: more than 1024 query heads or 256 KV heads");
   unsupported(s.past_tokens + s.tokens <= (1U << 23), "KV attention: a prompt's context is at most 2^23 tokens");
+  unsupported(s.tokens <= kPrefillMaxTokens, "KV attention: a chunk is at most 65535 * 128 tokens");
   require(s.max_context_tokens <= kUnbounded, "KV attention: max_context_tokens exceeds 2^31");
 }
 

@@ -144,6 +144,7 @@ struct BatchedDecodeArgs {
 void launch_batched_decode_attention(const BatchedDecodeArgs &args, cudaStream_t stream);
 
 // ---- prefill attention (prefill_attention.cu) -----------------------------------------------
+constexpr std::uint32_t kPrefillMaxTokens = 65535U * 128U; // of a launch
 // Windowed form of the launch: a query at position q sees keys j <= q with j > q - window or j < sinks.
 struct PrefillWindow {
   std::uint32_t window; // 0: not windowed

@@ -59,6 +59,7 @@ constexpr int kHeadDim = 256;
 // Head counts are run-time values (the reference's prefill takes any query_heads that is a multiple of kv_heads,
 // cpp/kernels/qwen35_online_attention.cu:33-44), which is also what a head-sharded rank passes: its own slice.
 constexpr int kTileRows = 128;  // query rows per CTA
+static_assert(kPrefillMaxTokens == 65535U * kTileRows, "tiles of a launch");
 constexpr int kBlockKeys = 128; // keys per score tile
 constexpr int kHalfKeys = 64;   // keys per ring slot
 constexpr int kNarrowKeys = 32; // keys of a block of few sinks
@@ -2060,7 +2061,7 @@ extern "C" int rib200_debug_read_cta_trace(long long *host, std::size_t count) {
 #endif
 
 void launch_prefill_attention(const PrefillArgs &args, cudaStream_t stream) {
-  require(args.tokens <= 65535U * kTileRows, "prefill attention: too many tokens for one launch");
+  require(args.tokens <= kPrefillMaxTokens, "prefill attention: too many tokens for one launch");
   // Few items, each with many key blocks (a short chunk against a long past): two CTAs share an item's keys.
   // Otherwise two query heads of one KV head form a pair; an odd group size keeps the single-CTA form.
   int device = 0;

@@ -421,8 +421,9 @@ Rib200Status rib200_online_attention_decode_early_kv_fetch(const void *query, co
  * the block's first row.  Outputs are out = (attention) * sigmoid(gate).
  * Activations (query, key, value, gate, output) are BF16 or FP32; a prompt call rounds FP32 queries to BF16, and FP32
  * keys and values to the cache's type; a single-token call rounds keys and values alone.  A prompt call rounds weights to
- * BF16, and counts gates under -40 as -40; a single-token call over an 8-bit cache keeps 2^-22 of a weight, or 2^-40 of the
- * head's largest product of a weight and its block's V scale if that is more, in place of the weight times its scale.
+ * BF16; a single-token call over an 8-bit cache keeps 2^-22 of a weight, or 2^-40 of the head's largest product of a weight and
+ * its block's V scale if that is more, in place of the weight times its scale.  Gates under -87 may count as minus infinity,
+ * and a gate that is not a number makes its output one.
  * Rows that are seen should be finite.  In a BF16 cache an infinity or a not-a-number counts as itself in a single-token call:
  * a logit of minus infinity is a weight of zero, an infinite value an infinite output in its dim.  A prompt call takes
  * 128 queries and 128 keys at a time and weights of zero for what is hidden: such a value may make its dim a not-a-number in

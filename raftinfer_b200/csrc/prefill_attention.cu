@@ -511,17 +511,19 @@ __device__ __forceinline__ float sigmoid_for_bf16(float x) {
   return fmaf(0.5F, t, 0.5F);
 }
 
-// Two of them with one reciprocal: 1 / a = b * (1 / (a b)).  Gates below -40 count as -40 (4e-18), which keeps a b finite.
+// Two of them with one reciprocal: 1 / a = b * (1 / (a b)), for x and y of kPairedGate or more, which keeps a b finite.
+constexpr float kPairedGate = -40.0F;
 __device__ __forceinline__ void fast_sigmoid2(float x, float y, float &sx, float &sy) {
-  const float a = 1.0F + fast_exp2(fmaxf(x, -40.0F) * -1.4426950408889634F);
-  const float b = 1.0F + fast_exp2(fmaxf(y, -40.0F) * -1.4426950408889634F);
+  const float a = 1.0F + fast_exp2(x * -1.4426950408889634F);
+  const float b = 1.0F + fast_exp2(y * -1.4426950408889634F);
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(a * b));
   sx = b * r;
   sy = a * r;
 }
 
-// 1 / (1 + e^-x) through ex2 and an approximate reciprocal (relative error ~1e-6, far below BF16 resolution)
+// 1 / (1 + e^-x) through ex2 and an approximate reciprocal (relative error ~1e-6, far below BF16 resolution; zero from
+// e^-x = 2^126 on, x = -87.3)
 __device__ __forceinline__ float fast_sigmoid(float x) {
   return __fdividef(1.0F, 1.0F + fast_exp2(x * -1.4426950408889634F));
 }
@@ -1417,15 +1419,28 @@ __global__ void __launch_bounds__(kThreads, 1)
             ok = mbar_wait(gate_bar, gate_parity, abort_flag);
             ok = __all_sync(0xFFFFFFFFU, ok);
             gate_parity ^= 1U;
+            __nv_bfloat162 lowest = __halves2bfloat162(CUDART_INF_BF16, CUDART_INF_BF16); // a not-a-number stays one
+            auto each_pair = [&](auto take) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const uint4 raw = *reinterpret_cast<const uint4 *>(box_row + ((i ^ (lane & 7)) << 4));
-              const std::uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
+              for (int i = 0; i < 8; ++i) {
+                const uint4 raw = *reinterpret_cast<const uint4 *>(box_row + ((i ^ (lane & 7)) << 4));
+                const std::uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-              for (int h = 0; h < 4; ++h) {
-                fast_sigmoid2(__uint_as_float(words[h] << 16), __uint_as_float(words[h] & 0xFFFF0000U),
-                              gates[8 * i + 2 * h], gates[8 * i + 2 * h + 1]);
+                for (int h = 0; h < 4; ++h) {
+                  take(words[h], gates[8 * i + 2 * h], gates[8 * i + 2 * h + 1]);
+                }
               }
+            };
+            each_pair([&](std::uint32_t word, float &sx, float &sy) {
+              lowest = __hmin2_nan(lowest, *reinterpret_cast<const __nv_bfloat162 *>(&word));
+              fast_sigmoid2(__uint_as_float(word << 16), __uint_as_float(word & 0xFFFF0000U), sx, sy);
+            });
+            // small gates and not-a-numbers: for all of the warp, one by one
+            if (__any_sync(0xFFFFFFFFU, !(__low2float(lowest) >= kPairedGate && __high2float(lowest) >= kPairedGate))) {
+              each_pair([&](std::uint32_t word, float &sx, float &sy) {
+                sx = fast_sigmoid(__uint_as_float(word << 16));
+                sy = fast_sigmoid(__uint_as_float(word & 0xFFFF0000U));
+              });
             }
             gates_asked = false;
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");

@@ -379,6 +379,15 @@ template <bool F32> __device__ __forceinline__ void load8(const void *base, std:
     }
   }
 }
+// x times a share or weight.  Over BF16 rows an infinity stays one where FP32 has only a zero left of a share that is more; 8-bit
+// rows hold none.
+template <bool EightBit> __device__ __forceinline__ float share_of(float x, float by) {
+  return EightBit || fabsf(x) <= 3.4028234663852886e38F ? x * by : x;
+}
+template <bool EightBit> __device__ __forceinline__ float4 share_of(float4 v, float by) {
+  return make_float4(share_of<EightBit>(v.x, by), share_of<EightBit>(v.y, by), share_of<EightBit>(v.z, by),
+                     share_of<EightBit>(v.w, by));
+}
 template <bool F32> __device__ __forceinline__ float4 load4(const void *base, std::size_t index) {
   if constexpr (F32) {
     return *reinterpret_cast<const float4 *>(static_cast<const float *>(base) + index);
@@ -629,7 +638,8 @@ __device__ __noinline__ void plain_part(const DecodeParams &p, std::uint32_t seq
         sum[h] = fmaf(sum[h], keep, weight);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          out[h][e] = fmaf(weight, v[e], out[h][e] * keep);
+          const float term = logit > -INFINITY ? share_of<false>(v[e], weight) : weight * v[e];
+          out[h][e] = share_of<false>(out[h][e], keep) + term;
         }
       }
     }
@@ -1105,9 +1115,10 @@ __global__ void __launch_bounds__(Shape<EightBit>::kWarps * 32, Shape<EightBit>:
 #pragma unroll
       for (std::uint32_t w = 0; w < kWarps; ++w) {
         const float share = warp_sum[w * kGroup + h] * fast_exp2(warp_max[w * kGroup + h] - top);
-        const float4 v = *reinterpret_cast<const float4 *>(warp_out + (w * kGroup + h) * kMergePitch + dim0);
+        const float4 v = share_of<EightBit>(
+            *reinterpret_cast<const float4 *>(warp_out + (w * kGroup + h) * kMergePitch + dim0), share);
         sum += share;
-        out.x += v.x * share; out.y += v.y * share; out.z += v.z * share; out.w += v.w * share;
+        out.x += v.x; out.y += v.y; out.z += v.z; out.w += v.w;
       }
       const float inverse = 1.0F / sum;
       out = make_float4(out.x * inverse, out.y * inverse, out.z * inverse, out.w * inverse);
@@ -1144,7 +1155,7 @@ __global__ void __launch_bounds__(Shape<EightBit>::kWarps * 32, Shape<EightBit>:
 // block for every cut between two CTAs, which serves the row that the cut is the first one in, 64 threads a query head.  A
 // thread has four dims.
 constexpr std::uint32_t kCombineGroups = 8;
-template <bool F32>
+template <bool F32, bool EightBit>
 __global__ void __launch_bounds__(kCombineGroups * 64) kv_combine_kernel(const __grid_constant__ DecodeParams p) {
   __shared__ float group_max[kCombineGroups], group_sum[kCombineGroups];
   __shared__ float4 group_out[kCombineGroups][64];
@@ -1227,10 +1238,8 @@ __global__ void __launch_bounds__(kCombineGroups * 64) kv_combine_kernel(const _
         const float next = fmaxf(top, m[j]);
         const float keep = fast_exp2(top - next), take = l[j] * fast_exp2(m[j] - next);
         sum = sum * keep + take;
-        out.x = out.x * keep + v[j].x * take;
-        out.y = out.y * keep + v[j].y * take;
-        out.z = out.z * keep + v[j].z * take;
-        out.w = out.w * keep + v[j].w * take;
+        const float4 kept = share_of<EightBit>(out, keep), taken = share_of<EightBit>(v[j], take);
+        out = make_float4(kept.x + taken.x, kept.y + taken.y, kept.z + taken.z, kept.w + taken.w);
         top = next;
       }
     }
@@ -1255,10 +1264,8 @@ __global__ void __launch_bounds__(kCombineGroups * 64) kv_combine_kernel(const _
     for (std::uint32_t i = 0; i < kCombineGroups; ++i) {
       const float weight = fast_exp2(group_max[i] - top);
       sum += group_sum[i] * weight;
-      out.x += group_out[i][lane].x * weight;
-      out.y += group_out[i][lane].y * weight;
-      out.z += group_out[i][lane].z * weight;
-      out.w += group_out[i][lane].w * weight;
+      const float4 v = share_of<EightBit>(group_out[i][lane], weight);
+      out.x += v.x; out.y += v.y; out.z += v.z; out.w += v.w;
     }
   }
   const float inverse = 1.0F / sum;
@@ -1291,7 +1298,7 @@ template <bool F32, bool EightBit> void launch(DecodeParams p, cudaStream_t stre
   launch_programmatic(kv_decode_kernel<F32, EightBit>, dim3(p.ctas), dim3(S::kWarps * 32), S::kSmemBytes, stream,
                       "KV decode launch", p);
   const dim3 grid = p.by_rows != 0 ? dim3(rows, p.group) : dim3(p.ctas - 1);
-  launch_programmatic(kv_combine_kernel<F32>, grid, dim3(64 * (p.by_rows != 0 ? kCombineGroups : p.group)), 0, stream,
+  launch_programmatic(kv_combine_kernel<F32, EightBit>, grid, dim3(64 * (p.by_rows != 0 ? kCombineGroups : p.group)), 0, stream,
                       "KV decode combine launch", p);
 }
 

@@ -228,6 +228,21 @@ def test_values_that_are_infinite(dtype, paged, lengths):
 
 
 @DTYPES
+@pytest.mark.parametrize("lengths", [LENGTHS, [40 + 53 * i for i in range(30)]], ids=["few", "many"])
+def test_an_infinite_value_under_a_weight_that_32_bits_do_not_hold(dtype, lengths):
+    """A weight of e^-150 is not zero: in front of the tokens that have all of the weight, behind them, and in the new token."""
+    def edit(i, keys, values):
+        n = keys.shape[1]
+        for at, dim in ((0, 3), (n // 2, 4), (n - 1, 5)):
+            keys[:, at, 0], values[:, at, dim] = -300.0, math.inf
+        values[:, n // 3, 5] = -math.inf
+
+    b = Rows(K.KV_BF16, lengths, dtype, 290, edit, kv_heads=2)
+    b.run()
+    b.check_range()
+
+
+@DTYPES
 def test_infinities_that_the_window_hides(dtype):
     def edit(i, keys, values):
         n = keys.shape[1]

@@ -436,7 +436,8 @@ enum { RIB200_KV8_BLOCK_TOKENS = 16, RIB200_KV8_BLOCK_BYTES = 4112 };
 
 /* Bytes of one sequence's cache; a page is rib200_kv_cache_bytes(kv_heads, 256, ...).  BF16 or E4M3. */
 Rib200Status rib200_kv_cache_bytes(size_t kv_heads, size_t max_context_tokens, uint8_t cache_dtype, size_t *bytes);
-/* Workspace of the prompt calls: the rows that the chunk sees, in BF16.  0 for a contiguous BF16 cache (paged == 0). */
+/* Workspace of the prompt calls: the rows that the chunk sees, in BF16, which is twice the bytes that an 8-bit cache holds them in.
+ * 0 for a contiguous BF16 cache (paged == 0). */
 Rib200Status rib200_kv_prefill_workspace_bytes(const Rib200AttentionShape *shape, size_t window_tokens,
                                                size_t sink_tokens, uint8_t cache_dtype, int32_t paged, size_t *bytes);
 /* Workspace of the single-token calls, the same for every batch and length. */
@@ -484,7 +485,7 @@ Rib200Status rib200_kv_paged_decode(const void *query, const void *key, const vo
  * `output` may be `input` itself where their types are the same; other overlaps are not allowed.
  * output_dtype == dtype: output = y, scales NULL, group_columns 0.  RIB200_DTYPE_E4M3: output holds codes [rows][columns]
  * and scales (FP32) [rows][columns / group_columns], the powers of two of the 8-bit cache for each group of 32 or 128
- * columns of a row; group_columns == 0 is one scale for the row.  A code is the value rounded once.
+ * columns of a row; group_columns == 0 is one scale for the row.  A code is the value rounded once, in rows of any magnitude.
  * dtype FP32, BF16 or FP16; weight FP32 or BF16; columns a multiple of 8 (of group_columns) up to 16384. */
 Rib200Status rib200_residual_rms_norm(const void *input, const void *residual, const void *weight, void *output,
                                       float *scales, void *residual_out, size_t rows, size_t columns,

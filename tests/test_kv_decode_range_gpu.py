@@ -253,3 +253,11 @@ def test_infinities_that_the_window_hides(dtype):
     b = Rows(K.KV_BF16, [700, 77, 300], dtype, 280, edit, kv_heads=1, window=50, sinks=5)
     b.run()
     b.check_range()
+
+
+@pytest.mark.parametrize("kind", [K.KV_BF16, K.KV_E4M3], ids=["bf16", "e4m3"])
+def test_one_long_context_among_short_ones(kind):
+    """Too many rows to cut each by itself: the long one's rows are put together from dozens of parts."""
+    b = Rows(kind, [500] * 6 + [30001] + [500 + 7 * i for i in range(13)], K.DTYPE_F32, 300, lambda i, keys, values: None, kv_heads=2)
+    b.run()
+    b.check_range()
